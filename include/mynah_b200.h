@@ -486,6 +486,128 @@ int mynah_b200_codec_decode_partial(void *codec, const unsigned *codes, size_t f
 int mynah_b200_codec_time(void *codec, const unsigned *codes, size_t frames, int repeats,
                           float *ms_per_decode, char *error, size_t cap);
 
+/* ---- beam decoding ------------------------------------------------------------
+ * No counterpart in the reference, which follows one candidate per request.  Three device
+ * operators on the self K/V of a batch whose lanes are the beams (or just the streams) of its
+ * requests, lane = request * beams + beam:
+ *
+ *   mynah_b200_lane_attention  one new row per lane attends a prefix that lanes share, the
+ *                              lane's own cached rows and itself, and is appended
+ *   mynah_b200_beam_select     picks every request's best continuations
+ *   mynah_b200_beam_reorder    gives the picked beams their parents' own rows
+ *
+ * Pointers named dev_* are memory of the backend's device, from mynah_cuda_dev_alloc or any
+ * other allocation there.  The calls enqueue on the backend's stream and return; they neither
+ * allocate nor synchronize, so they may be captured into a CUDA graph, and they leave the
+ * calling thread's current device as it was.  Lengths, slots, prefixes, parents and the live
+ * counts are read on the device when the work runs: a captured graph follows their current
+ * values.  Every operator computes the same in strict and in fast mode. */
+
+/* K and V rows of `slots` slots: slot_stride elements apart, `capacity` rows each,
+ * row_stride apart, `width` elements per row.  type is MYNAH_B200_F32 or MYNAH_B200_F16.
+ * dev_k and dev_v start on 16 bytes, and strides and width are multiples of 16 bytes (slots
+ * and layers may interleave: the decoder keeps [slot][layer][capacity][width]). */
+typedef struct {
+    int type;
+    void *dev_k, *dev_v;
+    size_t slots, capacity, width, row_stride, slot_stride;
+    size_t layers, layer_stride;  /* _beam_reorder moves `layers` layers, layer_stride elements
+                                   * apart; _lane_attention works on the one at dev_k / dev_v */
+} mynah_b200_lane_cache;
+
+/* Single-token attention, the batched form of mynah_cuda_self_attention_dev with a shared
+ * prefix and a window.  Lane b has its query, key and value row in dev_qkv, n = dev_length[b]
+ * own rows cached in its slot, and the P rows of its prefix in front of them.  It attends
+ * rows 0 .. P + n of the joined sequence (row P + n is the new one), or, with window > 0, of
+ * these the rows j < sinks and j > P + n - window:
+ *     out = sum_j softmax_j(scale * q.k_j) v_j
+ * in 32-bit arithmetic; the new K/V row is rounded to the cache's type and appended before it
+ * is attended.  Lengths are not advanced.
+ *
+ * Own row r lies in cache row r, and where a window makes the cache a ring in row
+ * keep + (r - keep) % (capacity - keep) for r >= keep = max(0, sinks - P); a windowed cache
+ * holds at least window + sinks rows, and a lane's prefix keeps its length while the ring turns.
+ * Without a window a lane whose length has reached the capacity, and with or without one a
+ * lane whose slot is not below `slots`, is left out (its output and cache stay as they were)
+ * and the next mynah_cuda_sync reports it.  A slot may appear once per call.  Rows of the
+ * cache that a lane does not see may hold anything.
+ *
+ * Limits: 1 .. 1024 lanes, 1 .. 64 heads, head_width up to 128 in multiples of 16 bytes of the
+ * cache's type, lanes * (capacity + prefix_capacity) < 2^32. */
+typedef struct {
+    size_t lanes, heads, head_width;   /* cache.width = heads * head_width */
+    float scale;
+    const float *dev_qkv;              /* [lanes] rows of q, k, v (heads * head_width floats each) */
+    size_t qkv_stride;                 /* floats between rows, >= 3 * heads * head_width */
+    mynah_b200_lane_cache cache;
+    const unsigned *dev_slot;          /* [lanes], or NULL: lane b owns slot b */
+    const unsigned *dev_length;        /* [lanes] own rows already cached */
+    size_t prefixes;                   /* 0: no lane has one, and the fields below are not read */
+    const void *dev_prefix_k, *dev_prefix_v;   /* rows of the cache's type, 16-byte aligned */
+    size_t prefix_capacity, prefix_row_stride, prefix_stride; /* rows; elements between rows, between prefixes */
+    const unsigned *dev_prefix_length; /* [prefixes] rows in use (at most prefix_capacity count) */
+    const unsigned *dev_lane_prefix;   /* [lanes], a value not below `prefixes`: none; NULL: prefix 0 */
+    size_t window, sinks;              /* window 0: every row */
+    const unsigned *dev_live;          /* lanes in use, or NULL: all; the others are left as they are */
+    float *dev_out;                    /* [lanes] rows of heads * head_width floats */
+    size_t out_stride;
+    float *dev_workspace;              /* 16-byte aligned; calls that may overlap need their own */
+    size_t workspace_floats;           /* at least mynah_b200_lane_attention_workspace */
+} mynah_b200_lane_attention_args;
+/* Floats of workspace a call of these sizes needs; 0 when the sizes are outside the limits. */
+size_t mynah_b200_lane_attention_workspace(const void *state, size_t lanes, size_t heads, size_t head_width,
+                                           size_t prefixes, size_t prefix_capacity);
+int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args *args, char *error, size_t cap);
+
+/* The best `beams` continuations of every request, by the rule of mynah_cuda_argmax_dev: the
+ * tokens below codebook_size, and eos_id where dev_allow_eos[request] is nonzero, may be
+ * picked.  With s_b the score of beam b, x_b its logits and lse_b the logarithm of the sum of
+ * exp(x_b) over the tokens that may be picked, token t continues beam b with the score
+ * s_b + x_bt - lse_b; a finished beam (dev_done) has one continuation, eos_id with s_b.
+ * Scores are formed and compared in 64 bits and stored in 32.  Order: higher score, lower
+ * beam, higher logit, lower token.  A logit that is NaN or -inf, and a continuation whose
+ * score is (a beam of score -inf is dead), is never picked; a place for which nothing is left
+ * gets score -inf, token 0 and its own index as parent.  A finished beam that is picked, and
+ * a beam whose token is eos_id, is done.  dev_score_out may be dev_score and dev_done_out
+ * dev_done; the other arrays are distinct.
+ * Limits: 1 .. 16 beams, vocab < 2^30, logits 4-byte aligned. */
+typedef struct {
+    const float *dev_logits;           /* [requests * beams] rows */
+    size_t requests, beams, vocab, logits_stride;
+    size_t codebook_size, eos_id;      /* codebook_size <= vocab; an eos_id >= vocab is never picked */
+    const int *dev_allow_eos;          /* [requests], or NULL: allowed */
+    const float *dev_score;            /* [requests * beams] */
+    const unsigned *dev_done;          /* [requests * beams], or NULL: none is */
+    const unsigned *dev_live;          /* requests in use, or NULL: all; the others are left as they are */
+    float *dev_score_out;              /* [requests * beams], as the following */
+    unsigned *dev_token, *dev_parent;  /* parent: beam index within the request */
+    unsigned *dev_done_out;            /* or NULL */
+} mynah_b200_beam_select_args;
+int mynah_b200_beam_select(void *state, const mynah_b200_beam_select_args *args, char *error, size_t cap);
+
+/* Own rows 0 .. min(dev_length[parent], capacity) - 1 of every beam become its parent's, in
+ * place, for K and V of all layers (a cache used as a ring moves whole); rows behind them
+ * stay.  A parent that is not a beam of the request, or a slot that is not below `slots`,
+ * moves nothing.  dev_length_out receives every lane's new length; it is an array of its own.
+ * Limits: 1 .. 16 beams, requests and 2 * layers up to 65535. */
+typedef struct {
+    mynah_b200_lane_cache cache;
+    size_t requests, beams;
+    const unsigned *dev_slot;          /* [requests * beams], or NULL: lane b owns slot b */
+    const unsigned *dev_parent;        /* [requests * beams] beam index within the request */
+    const unsigned *dev_length;        /* [requests * beams] */
+    unsigned *dev_length_out;          /* or NULL */
+    const unsigned *dev_live;          /* requests in use, or NULL: all */
+} mynah_b200_beam_reorder_args;
+int mynah_b200_beam_reorder(void *state, const mynah_b200_beam_reorder_args *args, char *error, size_t cap);
+
+/* The same for a decoder's slots (HOST arrays): lane request * beams + beam lives in slot
+ * slots[lane], each slot once; parents[lane] is the beam it continues.  Self K/V of all layers
+ * and the slots' lengths follow; cross K/V stay (the beams of a request share their text).
+ * Synchronous. */
+int mynah_b200_decoder_reorder(void *decoder, const unsigned *slots, const unsigned *parents, size_t requests,
+                               size_t beams, char *error, size_t cap);
+
 /* Bytes of weights one step reads, and of KV one slot at `length` reads. */
 size_t mynah_b200_decoder_weight_bytes(const void *decoder);
 size_t mynah_b200_decoder_kv_bytes(const void *decoder, size_t length);

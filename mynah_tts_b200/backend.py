@@ -189,11 +189,84 @@ class Backend:
              n, None if bias is None else fp(bias), None if ln_gain is None else fp(ln_gain))
         return out
 
+    # ---- beam decoding ---------------------------------------------------------
+    # The bind_* methods fill a call's descriptor once and return a function that makes the
+    # call: device addresses are DeviceBuffers or integers, and what lies there is read when
+    # the call runs.  The plain methods make one call.
+    @staticmethod
+    def lane_cache(cache_type, k, v, slots: int, capacity: int, width: int, row_stride: int | None = None,
+                   slot_stride: int | None = None, layers: int = 1, layer_stride: int = 0) -> capi.LaneCache:
+        """K and V rows of `slots` slots (mynah_b200_lane_cache); cache_type "f32" or "f16",
+        strides in elements, by default contiguous."""
+        row_stride = width if row_stride is None else row_stride
+        slot_stride = capacity * row_stride if slot_stride is None else slot_stride
+        kind = QUANT[cache_type] if isinstance(cache_type, str) else int(cache_type)
+        return capi.LaneCache(kind, _a(k), _a(v), slots, capacity, width, row_stride, slot_stride, layers, layer_stride)
+
+    def lane_attention_workspace(self, lanes: int, heads: int, head_width: int, prefixes: int = 0,
+                                 prefix_capacity: int = 0) -> int:
+        """Floats of workspace a lane_attention of these sizes needs."""
+        return int(self.lib.mynah_b200_lane_attention_workspace(self.state, lanes, heads, head_width, prefixes,
+                                                                prefix_capacity))
+
+    def bind_lane_attention(self, cache: capi.LaneCache, *, lanes: int, heads: int, head_width: int, scale: float, qkv,
+                            length, out, workspace, workspace_floats: int, qkv_stride: int | None = None,
+                            out_stride: int | None = None, slot=None, prefixes: int = 0, prefix_k=None, prefix_v=None,
+                            prefix_capacity: int = 0, prefix_row_stride: int | None = None,
+                            prefix_stride: int | None = None, prefix_length=None, lane_prefix=None, window: int = 0,
+                            sinks: int = 0, live=None):
+        """One new row per lane over a shared prefix, the lane's own rows and itself."""
+        width = heads * head_width
+        row = width if prefix_row_stride is None else prefix_row_stride
+        args = capi.LaneAttentionArgs(
+            lanes, heads, head_width, scale, _a(qkv), 3 * width if qkv_stride is None else qkv_stride, cache, _a(slot),
+            _a(length), prefixes, _a(prefix_k), _a(prefix_v), prefix_capacity, row,
+            prefix_capacity * row if prefix_stride is None else prefix_stride, _a(prefix_length), _a(lane_prefix), window,
+            sinks, _a(live), _a(out), width if out_stride is None else out_stride, _a(workspace), workspace_floats)
+        return self._bound(self.lib.mynah_b200_lane_attention, args)
+
+    def bind_beam_select(self, *, logits, requests: int, beams: int, vocab: int, codebook_size: int, eos_id: int, score,
+                         score_out, token, parent, logits_stride: int | None = None, allow_eos=None, done=None,
+                         done_out=None, live=None):
+        """The best `beams` continuations of every request."""
+        args = capi.BeamSelectArgs(
+            _a(logits), requests, beams, vocab, vocab if logits_stride is None else logits_stride, codebook_size, eos_id,
+            _a(allow_eos), _a(score), _a(done), _a(live), _a(score_out), _a(token), _a(parent), _a(done_out))
+        return self._bound(self.lib.mynah_b200_beam_select, args)
+
+    def bind_beam_reorder(self, cache: capi.LaneCache, *, requests: int, beams: int, parent, length, length_out=None,
+                          slot=None, live=None):
+        """The picked beams' own rows, in place."""
+        args = capi.BeamReorderArgs(cache, requests, beams, _a(slot), _a(parent), _a(length), _a(length_out), _a(live))
+        return self._bound(self.lib.mynah_b200_beam_reorder, args)
+
+    def lane_attention(self, cache: capi.LaneCache, **kw):
+        self.bind_lane_attention(cache, **kw)()
+
+    def beam_select(self, **kw):
+        self.bind_beam_select(**kw)()
+
+    def beam_reorder(self, cache: capi.LaneCache, **kw):
+        self.bind_beam_reorder(cache, **kw)()
+
+    def _bound(self, fn, args):
+        err, ref = C.create_string_buffer(capi.ERR_CAP), C.byref(args)
+
+        def step():
+            if fn(self.state, ref, err, capi.ERR_CAP) != 0:
+                raise MynahB200Error(err.value.decode(errors="replace") or f"{fn.__name__} failed")
+        return step
+
 
 def _p(dev):
     if isinstance(dev, DeviceBuffer):
         return dev.ptr
     return dev
+
+
+def _a(dev):
+    """A device address as a structure field: an integer, or None for an array left out."""
+    return dev.ptr.value if isinstance(dev, DeviceBuffer) else dev
 
 
 class MatrixPool:
@@ -458,6 +531,16 @@ class Decoder:
         v = np.empty_like(k)
         call(capi.lib().mynah_b200_decoder_slot_read_kv, self.handle, slot, fp(k), fp(v))
         return k, v
+
+    def reorder(self, slots, parents, beams: int):
+        """Self K/V and lengths of the slots follow the picked beams: lane request * beams + beam
+        lives in slots[lane] and continues beam parents[lane] of its request."""
+        slots = np.ascontiguousarray(slots, np.uint32)
+        parents = np.ascontiguousarray(parents, np.uint32)
+        if slots.ndim != 1 or slots.shape != parents.shape or slots.size % beams != 0:
+            raise ValueError("slots and parents hold requests * beams entries each")
+        call(capi.lib().mynah_b200_decoder_reorder, self.handle, slots.ctypes.data_as(capi.c_uint_p),
+             parents.ctypes.data_as(capi.c_uint_p), slots.size // beams, beams)
 
     def set_layers(self, n: int):
         call(capi.lib().mynah_b200_decoder_set_layers, self.handle, n)

@@ -102,6 +102,33 @@ class Request(C.Structure):
                 ("admitted_at", sz)]
 
 
+class LaneCache(C.Structure):
+    _fields_ = [("type", C.c_int), ("dev_k", C.c_void_p), ("dev_v", C.c_void_p)] + [(n, sz) for n in (
+        "slots", "capacity", "width", "row_stride", "slot_stride", "layers", "layer_stride")]
+
+
+class LaneAttentionArgs(C.Structure):
+    _fields_ = [("lanes", sz), ("heads", sz), ("head_width", sz), ("scale", C.c_float), ("dev_qkv", C.c_void_p),
+                ("qkv_stride", sz), ("cache", LaneCache), ("dev_slot", C.c_void_p), ("dev_length", C.c_void_p),
+                ("prefixes", sz), ("dev_prefix_k", C.c_void_p), ("dev_prefix_v", C.c_void_p), ("prefix_capacity", sz),
+                ("prefix_row_stride", sz), ("prefix_stride", sz), ("dev_prefix_length", C.c_void_p),
+                ("dev_lane_prefix", C.c_void_p), ("window", sz), ("sinks", sz), ("dev_live", C.c_void_p),
+                ("dev_out", C.c_void_p), ("out_stride", sz), ("dev_workspace", C.c_void_p), ("workspace_floats", sz)]
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [("dev_logits", C.c_void_p), ("requests", sz), ("beams", sz), ("vocab", sz), ("logits_stride", sz),
+                ("codebook_size", sz), ("eos_id", sz), ("dev_allow_eos", C.c_void_p), ("dev_score", C.c_void_p),
+                ("dev_done", C.c_void_p), ("dev_live", C.c_void_p), ("dev_score_out", C.c_void_p),
+                ("dev_token", C.c_void_p), ("dev_parent", C.c_void_p), ("dev_done_out", C.c_void_p)]
+
+
+class BeamReorderArgs(C.Structure):
+    _fields_ = [("cache", LaneCache), ("requests", sz), ("beams", sz), ("dev_slot", C.c_void_p),
+                ("dev_parent", C.c_void_p), ("dev_length", C.c_void_p), ("dev_length_out", C.c_void_p),
+                ("dev_live", C.c_void_p)]
+
+
 MATMUL_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, c_float_p, c_float_p, sz, sz, sz, c_float_p, c_float_p,
                         C.c_char_p, sz)
 SGEMM_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.c_int, sz, sz, sz, C.c_float, c_float_p, sz,
@@ -212,6 +239,11 @@ SIGNATURES = {
     "mynah_b200_profile_class_name": (C.c_char_p, [sz]),
     "mynah_b200_self_attention_static": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, sz, sz, sz, sz, sz,
                                                    C.c_float, C.c_void_p, C.c_void_p, _E]),
+    "mynah_b200_lane_attention_workspace": (sz, [C.c_void_p, sz, sz, sz, sz, sz]),
+    "mynah_b200_lane_attention": (C.c_int, [C.c_void_p, C.POINTER(LaneAttentionArgs), _E]),
+    "mynah_b200_beam_select": (C.c_int, [C.c_void_p, C.POINTER(BeamSelectArgs), _E]),
+    "mynah_b200_beam_reorder": (C.c_int, [C.c_void_p, C.POINTER(BeamReorderArgs), _E]),
+    "mynah_b200_decoder_reorder": (C.c_int, [C.c_void_p, c_uint_p, c_uint_p, sz, sz, _E]),
     "mynah_b200_decoder_weight_bytes": (sz, [C.c_void_p]),
     "mynah_b200_decoder_kv_bytes": (sz, [C.c_void_p, sz]),
 }

@@ -101,6 +101,7 @@ typedef struct mb_decoder {
     size_t *slot_len;           /* host mirror of every slot's length */
     int *d_mem_len;             /* [slots] text states of the request in each slot (<= T) */
     size_t *slot_mem;           /* host mirror */
+    unsigned *d_beam;           /* [3][slots] slot, parent and length of the lanes of a _reorder */
     float *pf_mem, *pf_nrm, *pf_kv;   /* prefill scratch: [T][W], [T][W], [T][2xw] */
     void *pf_planes;                  /* fast mode: f16 hi/lo planes of the normalized text states, [2][T][W] */
     mb_local local;             /* layers == 0: not attached */
@@ -222,7 +223,7 @@ void mynah_b200_decoder_destroy(void *decoder) {
     void *dev[] = {d->position, d->norm_out, d->emb, (void *)d->d_tables, d->heads_b, d->self_k,
                    d->self_v, d->cross_k, d->cross_v, d->x, d->nrm, d->qkv, d->attn, d->q_x,
                    d->xctx, d->hidden, d->out, d->rows_in, d->logits, d->qx, d->sx, d->xsplit, d->row_planes, d->cand_v, d->cand_i, d->cand_counters, d->partials,
-                   d->counters, d->d_stage_in, d->d_stage_out, d->d_eos_frame, d->d_min_frames,
+                   d->counters, d->d_stage_in, d->d_stage_out, d->d_eos_frame, d->d_min_frames, d->d_beam,
                    d->d_history, d->d_mem_len, d->pf_mem, d->pf_nrm, d->pf_kv, d->pf_planes};
     for (size_t i = 0; i < sizeof(dev) / sizeof(dev[0]); ++i) cudaFree(dev[i]);
     void *pinned[] = {d->h_rows, d->h_out, d->h_stage_in, d->h_stage_out, d->h_ints, d->h_table};
@@ -499,6 +500,7 @@ int mynah_b200_decoder_create(void *state, const mynah_b200_decoder_desc *desc, 
         d->d_tokens = d->d_stage_out + 4u;
     }
     D_TRY(dmalloc((void **)&d->d_min_frames, sizeof(int), error, cap));
+    D_TRY(dmalloc((void **)&d->d_beam, 3u * d->slots * sizeof(unsigned), error, cap));
     if (ok) {
         D_TRY(mb_cuda((int)cudaMemset(d->counters, 0, n_counters * sizeof(unsigned)), "memset", error, cap));
         D_TRY(mb_cuda((int)cudaMemset(d->d_min_frames, 0, sizeof(int)), "memset", error, cap));
@@ -1177,6 +1179,68 @@ int mynah_b200_decoder_slot_read_kv(void *decoder, size_t slot, float *self_k, f
     MB_TRY(cudaStreamSynchronize(d->st->stream), "cudaStreamSynchronize");
     MB_TRY(cudaMemcpy(self_k, d->self_k + slot * n, n * sizeof(float), cudaMemcpyDeviceToHost), "read K");
     MB_TRY(cudaMemcpy(self_v, d->self_v + slot * n, n * sizeof(float), cudaMemcpyDeviceToHost), "read V");
+    mb_clear_error(error, cap);
+    return 0;
+}
+
+/* The self K/V and lengths of a request's slots follow the beams that were picked. */
+int mynah_b200_decoder_reorder(void *decoder, const unsigned *slots, const unsigned *parents, size_t requests,
+                               size_t beams, char *error, size_t cap) {
+    mb_decoder *d = (mb_decoder *)decoder;
+    if (d == NULL || slots == NULL || parents == NULL || requests == 0 || beams == 0 || beams > MB_BEAM_MAX ||
+        requests > d->slots / beams || requests > 65535u) {
+        mb_set_error(error, cap, "reorder takes 1..16 beams per request and at most the decoder's slots");
+        return -1;
+    }
+    const size_t n = requests * beams;
+    unsigned *lanes = (unsigned *)malloc(3u * n * sizeof(unsigned));
+    unsigned char *used = (unsigned char *)calloc(d->slots, 1u);
+    const char *wrong = lanes == NULL || used == NULL ? "out of memory reordering slots" : NULL;
+    for (size_t b = 0; b < n && wrong == NULL; ++b) {
+        if (slots[b] >= d->slots) wrong = "decoder slot out of range";
+        else if (used[slots[b]]) wrong = "a slot may appear once per reorder";
+        else if (parents[b] >= beams) wrong = "parent beam out of range";
+        else used[slots[b]] = 1;
+    }
+    for (size_t b = 0; b < n && wrong == NULL; ++b) {
+        lanes[b] = slots[b];
+        lanes[n + b] = parents[b];
+        lanes[2u * n + b] = (unsigned)d->slot_len[slots[b]];
+    }
+    free(used);
+    if (wrong != NULL) {
+        free(lanes);
+        mb_set_error(error, cap, wrong);
+        return -1;
+    }
+    mb_beam_reorder_args a;
+    memset(&a, 0, sizeof(a));
+    a.cache.type = MB_F32;
+    a.cache.k = d->self_k;
+    a.cache.v = d->self_v;
+    a.cache.slots = d->slots;
+    a.cache.capacity = d->capacity;
+    a.cache.width = a.cache.row_stride = d->width;
+    a.cache.layers = d->layers;
+    a.cache.layer_stride = d->capacity * d->width;
+    a.cache.slot_stride = d->layers * a.cache.layer_stride;
+    a.requests = requests;
+    a.beams = beams;
+    a.slot = d->d_beam;
+    a.parent = d->d_beam + n;
+    a.length = d->d_beam + 2u * n;
+    a.sm_count = d->st->sm_count;
+    cudaStream_t s = d->st->stream;
+    int rc = (int)cudaSetDevice(d->st->device);
+    if (rc == 0) rc = (int)cudaMemcpyAsync(d->d_beam, lanes, 3u * n * sizeof(unsigned), cudaMemcpyHostToDevice, s);
+    if (rc == 0) rc = mb_beam_reorder(&a, s);
+    if (rc == 0) rc = (int)cudaStreamSynchronize(s);
+    if (rc == 0) {
+        d->st->launches += 1;
+        for (size_t b = 0; b < n; ++b) d->slot_len[slots[b]] = lanes[2u * n + b / beams * beams + parents[b]];
+    }
+    free(lanes);
+    if (mb_cuda(rc, "reorder slots", error, cap) != 0) return -1;
     mb_clear_error(error, cap);
     return 0;
 }

@@ -363,6 +363,69 @@ int mb_cross_block_init(void);
 int mb_cross_block_supported(size_t width, size_t xw, size_t rows);
 int mb_cross_block(const mb_cross_block_args *args, mb_stream stream);
 
+/* ---- beam decoding (beam.cu, lane_attention.cu) --------------------------- */
+/* K and V rows of the slots of a batch: slots x capacity rows of `width` elements (MB_F32 or
+ * MB_F16), slot_stride and row_stride apart, for one layer or, layer_stride apart, several. */
+typedef struct {
+    int type;
+    void *k, *v;
+    size_t slots, capacity, width, row_stride, slot_stride, layers, layer_stride;
+} mb_lane_cache;
+
+enum { MB_BEAM_MAX = 16 };   /* beams of one request */
+
+typedef struct {
+    const float *logits;        /* [requests * beams][logits_stride] */
+    size_t requests, beams, codebook_size, eos_id, logits_stride;
+    int has_eos;                /* eos_id is a token of the vocabulary beyond codebook_size */
+    const int *allow_eos;       /* [requests] or NULL (allowed) */
+    const float *score;         /* [requests * beams] */
+    const unsigned *done;       /* [requests * beams] or NULL */
+    const unsigned *live;       /* requests in use, or NULL */
+    float *score_out;
+    unsigned *token, *parent, *done_out;   /* done_out may be NULL */
+} mb_beam_select_args;
+int mb_beam_select(const mb_beam_select_args *args, mb_stream stream);
+
+typedef struct {
+    mb_lane_cache cache;
+    size_t requests, beams;
+    const unsigned *slot;       /* [requests * beams] or NULL (identity) */
+    const unsigned *parent;     /* [requests * beams] */
+    const unsigned *length;     /* [requests * beams] */
+    unsigned *length_out;       /* or NULL */
+    const unsigned *live;
+    int sm_count;
+} mb_beam_reorder_args;
+int mb_beam_reorder(const mb_beam_reorder_args *args, mb_stream stream);
+
+enum { MB_LANES_MAX = 1024, MB_LANE_HEADS_MAX = 64, MB_LANE_HEAD_WIDTH_MAX = 128 };
+typedef struct {
+    size_t lanes, heads, head_width;
+    float scale;
+    const float *qkv;           /* [lanes][qkv_stride]: q, k, v */
+    size_t qkv_stride;
+    mb_lane_cache cache;
+    const unsigned *slot;       /* [lanes] or NULL */
+    const unsigned *length;     /* [lanes] */
+    const void *prefix_k, *prefix_v;
+    size_t prefixes, prefix_capacity, prefix_row_stride, prefix_stride;
+    const unsigned *prefix_length;   /* [prefixes] */
+    const unsigned *lane_prefix;     /* [lanes] or NULL (prefix 0) */
+    size_t window, sinks;       /* window 0: every row */
+    const unsigned *live;
+    float *out;
+    size_t out_stride;
+    float *workspace;           /* mb_lane_attention_floats() */
+    int *status;
+    int sm_count;
+    unsigned *launched;         /* incremented by the number of kernels the call enqueued */
+} mb_lane_attn_args;
+size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes, size_t prefix_capacity,
+                                int sm_count);
+int mb_lane_attention_init(void);
+int mb_lane_attention(const mb_lane_attn_args *args, mb_stream stream);
+
 #ifdef __cplusplus
 }
 #endif
