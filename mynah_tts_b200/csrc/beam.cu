@@ -20,48 +20,69 @@ namespace cg = cooperative_groups;
 //
 // Bound by reading the logits once.  A request is one thread-block cluster, so it is one
 // launch without scratch memory: the rows, or equal parts of them when there are few, are
-// dealt to the CTAs, each keeps the running maximum and sum of its row and finds the row's
-// best `beams` tokens, and the cluster's first CTA, into whose shared memory all results
-// are stored, ranks at most 256 continuations.
+// dealt to the CTAs, each keeps the running maximum and sum of its row and
+// finds the row's best `beams` tokens, and the cluster's first CTA, into whose shared memory
+// all results are stored, takes the best of at most 16 falling lists of 16.
 //
-// Best tokens of a part without sorting it: every group of eight threads knows the largest
-// key (logit, then lower token) it has seen; the K-th largest of these group maxima is a
-// lower bound of the K-th largest key, and only a few more than K keys reach it.  The threads
-// whose own maximum does are the only ones whose tokens are read again (by their whole warp).
+// Best tokens of a part without sorting it: each of 32 groups of threads knows the largest
+// logit it has seen; the K-th largest of these group maxima is a lower bound of the K-th
+// largest logit, and only a few more than K tokens reach it.  They are listed as they pass.
+// The bound is drawn again with 1, 2, 4, ... turns of the part seen, so about K log2(turns) tokens
+// are listed in all.  A list that is full all the same (thousands of equal logits, or logits
+// that rise along the vocabulary) is replaced by one pass over the part per place.
 //
 // Scores are formed in 64 bits: beams differ by less than a rounding of a 32-bit sum often
 // enough to change a pick.  The sums of exponentials are 32-bit per thread (at most a few
 // hundred terms, each off by 1e-7 of itself) and 64-bit across threads.
 
 constexpr int SEL_CLUSTER = 8;     // portable cluster size
-constexpr int SEL_CAP = 512;       // keys that may reach the bound before the slow path is taken
-constexpr int SEL_GROUPS = 64;     // threads / 8, at most
+constexpr int SEL_SHARE = 4;       // parts of one CTA, at most
+constexpr int SEL_THREADS = 1024, SEL_FIT_THREADS = 256;
+constexpr int SEL_HELD = 4;        // 16-byte pieces a thread takes in a turn, and holds of a short part (FIT)
+constexpr int SEL_CAP = 512;       // tokens listed of a part
+constexpr int SEL_PAD = MB_BEAM_MAX + 1;         // lists that lanes walk side by side: no common bank
+constexpr int SEL_LIST = MB_BEAM_MAX * SEL_PAD;
+
+// A long part goes through a ring in shared memory in which a thread fills and reads only its
+// own places, so the copies need no barrier: SEL_DEPTH turns of SEL_HELD pieces are under way,
+// 192 KB of an SM's one CTA.  (Two smaller CTAs per SM lost: the CTAs of a cluster are placed
+// in pairs on half as many SMs.)
+constexpr int SEL_DEPTH = 3;
+constexpr unsigned SEL_RING_BYTES = SEL_DEPTH * SEL_HELD * SEL_THREADS * sizeof(float4);
 
 struct SelPart {                   // what one part of a row found
-    float top;                     // running maximum, -inf if no token
+    float top;                     // maximum, -inf if no token
     float pad;
     double sum;                    // sum of exp(x - top)
+    double lse;                    // top + log(sum)
     unsigned long long key[MB_BEAM_MAX];
+};
+
+struct SelScratch {                // of one part while it is worked on
+    float group[32], bound;
+    double wsum[SEL_THREADS / 32];
+    float wtop[SEL_THREADS / 32];
+    unsigned n_reach;
+    unsigned long long reach[SEL_CAP], wkey[SEL_THREADS / 32];
 };
 
 struct SelSmem {
     SelPart part[MB_BEAM_MAX];     // first CTA: all parts of the request
-    unsigned long long group[SEL_GROUPS];
-    unsigned long long reach[SEL_CAP];
-    double wsum[16];
-    float wtop[16];
-    unsigned n_reach;
-    unsigned long long wkey[16];
-    double lse[MB_BEAM_MAX];
-    double score[MB_BEAM_MAX * MB_BEAM_MAX];
+    SelScratch work[SEL_SHARE];
+    double score[SEL_LIST];        // first CTA: the continuations of the request
+    unsigned long long order[SEL_LIST], key[SEL_LIST];
+    int taken[MB_BEAM_MAX];
 };
 
-// Order-preserving key of a logit and its token: larger logit first, then the lower token.
+// Order-preserving bits of a float.
+__device__ __forceinline__ unsigned sel_bits(float x) {
+    const unsigned u = __float_as_uint(x);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+// Key of a logit and its token: larger logit first, then the lower token; -0 and +0 are equal.
 // 0 is no key: NaN and -inf are not candidates.
 __device__ __forceinline__ unsigned long long sel_key(float x, unsigned token) {
-    const unsigned u = __float_as_uint(x + 0.0f);      // -0 and +0 are equal
-    const unsigned o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return ((unsigned long long)o << 32) | (0xffffffffu - token);
+    return ((unsigned long long)sel_bits(x + 0.0f) << 32) | (0xffffffffu - token);
 }
 __device__ __forceinline__ float sel_logit(unsigned long long key) {
     const unsigned o = (unsigned)(key >> 32);
@@ -71,12 +92,13 @@ __device__ __forceinline__ unsigned sel_token(unsigned long long key) { return 0
 
 __device__ __forceinline__ unsigned long long max_u64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
+// Tokens first .. last - 1 of a row as 16-byte pieces; piece v holds tokens origin + 4 v ...
 struct SelRange {
-    const float *row;              // token 0
-    const float4 *base;            // row + first, rounded down to 16 bytes
-    int first, last;               // tokens first .. last - 1
-    int shift;                     // tokens between base and row + first
-    int vecs;                      // 16-byte pieces that hold the range
+    const float *row;
+    const float4 *base;            // piece 0, 16-byte aligned
+    int first, last, origin;
+    int vecs;                      // pieces that hold the range
+    int whole_from, whole_to;      // pieces that lie inside it
 };
 
 __device__ __forceinline__ SelRange sel_range(const float *row, int first, int last) {
@@ -84,29 +106,71 @@ __device__ __forceinline__ SelRange sel_range(const float *row, int first, int l
     r.row = row;
     r.first = first;
     r.last = last;
-    r.shift = (int)((reinterpret_cast<uintptr_t>(row + first) & 15u) >> 2);
-    r.base = reinterpret_cast<const float4 *>(row + first - r.shift);
-    r.vecs = last > first ? (last - first + r.shift + 3) >> 2 : 0;
+    const int shift = (int)((reinterpret_cast<uintptr_t>(row + first) & 15u) >> 2);
+    r.origin = first - shift;
+    r.base = reinterpret_cast<const float4 *>(row + r.origin);
+    r.vecs = last > first ? (last - r.origin + 3) >> 2 : 0;
+    r.whole_from = min(r.vecs, shift ? 1 : 0);
+    r.whole_to = max(r.whole_from, last > first ? (last - r.origin) >> 2 : 0);
     return r;
 }
+__device__ __forceinline__ float drop_nan(float x) { return fmaxf(x, -INFINITY); }
+__device__ __forceinline__ float4 drop_nan(const float4 &x) {
+    return make_float4(drop_nan(x.x), drop_nan(x.y), drop_nan(x.z), drop_nan(x.w));
+}
+__device__ __forceinline__ float4 no_tokens() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
+
 // The four logits of piece v; tokens outside the range read as -inf and are not touched.
 __device__ __forceinline__ float4 sel_load(const SelRange &r, int v) {
-    const int t = r.first - r.shift + 4 * v;
+    if (v >= r.whole_from && v < r.whole_to) return r.base[v];
+    const int t = r.origin + 4 * v;
     float4 x;
-    if (t >= r.first && t + 4 <= r.last) {
-        x = r.base[v];
-    } else {
-        x.x = t >= r.first && t < r.last ? r.row[t] : -INFINITY;
-        x.y = t + 1 >= r.first && t + 1 < r.last ? r.row[t + 1] : -INFINITY;
-        x.z = t + 2 >= r.first && t + 2 < r.last ? r.row[t + 2] : -INFINITY;
-        x.w = t + 3 >= r.first && t + 3 < r.last ? r.row[t + 3] : -INFINITY;
-    }
+    x.x = t >= r.first && t < r.last ? r.row[t] : -INFINITY;
+    x.y = t + 1 >= r.first && t + 1 < r.last ? r.row[t + 1] : -INFINITY;
+    x.z = t + 2 >= r.first && t + 2 < r.last ? r.row[t + 2] : -INFINITY;
+    x.w = t + 3 >= r.first && t + 3 < r.last ? r.row[t + 3] : -INFINITY;
     return x;
 }
-__device__ __forceinline__ float drop_nan(float x) { return x == x ? x : -INFINITY; }
 
+// exp(x - top) for x <= top
 __device__ __forceinline__ float sel_exp(float x, float top) {
-    return exp2f(__fmul_rn(__fsub_rn(x, top), 1.4426950408889634f));
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fmul_rn(__fsub_rn(x, top), 1.4426950408889634f)));
+    return y;
+}
+
+// log(s) for a positive normal s, to 1e-12: with s = 2^e f and c near 1 / f in steps of 1/256
+// (64 intervals of f, Tang's table method), log s = e log 2 - log c + log(1 + r), r = f c - 1, |r| <
+// 0.013.  r is formed in 64 bits; of log(1 + r) = r - r^2/2 + ... only r needs them.  CUDA's
+// 64-bit log took 1.7 us here, which the whole cluster waits for; this takes a tenth.
+__constant__ double sel_log_c[64] = {      // -log(c), c = round(256 / (1 + (i + 0.5) / 64)) / 256
+    0.007843177461025893, 0.023716526617316044, 0.039845908547199674, 0.05211600113901402,
+    0.06871389254805181, 0.0813456394539524, 0.09844007281325252, 0.11145544092532282,
+    0.1246424452072766, 0.13800567301944372, 0.15154989812720093, 0.16528009093910292,
+    0.179201429457711, 0.19331931100349597, 0.20284319251475147, 0.2173012756899814,
+    0.22705745063534608, 0.24187253642048673, 0.2518726197550701, 0.26706278524904525,
+    0.27731928541623435, 0.2876820724517809, 0.3034304294199201, 0.31406882762497584,
+    0.32482161940123766, 0.33569129163814154, 0.3466804132137367, 0.3577916386388075,
+    0.36902771190573336, 0.38039147055604844, 0.39188584998178355, 0.39768296766610944,
+    0.4093790074293007, 0.42121346507630353, 0.43318965612301924, 0.4392319705789819,
+    0.4514272436728001, 0.4637730794950995, 0.4700036292457356, 0.48258241145259567,
+    0.4889316391312544, 0.5017523275603158, 0.5082248420659333, 0.5212969236332861,
+    0.5278976076646381, 0.5345421503833068, 0.5479651707154474, 0.5547448577008262,
+    0.561570822771226, 0.5753641449035618, 0.5823328142196552, 0.5893503868783018,
+    0.5964175541013942, 0.6107035113488707, 0.6179237593223578, 0.6251965186514375,
+    0.6325225587435105, 0.639902666041133, 0.6473376445286511, 0.6548283162578087,
+    0.6623755218931916, 0.6699801212784109, 0.6776429940239801, 0.6853650401178903,
+};
+__device__ __forceinline__ double sel_log(double s) {
+    const long long bits = __double_as_longlong(s);
+    const int e = (int)(bits >> 52) - 1023, i = (int)(bits >> 46) & 63;
+    const double f = __longlong_as_double((bits & 0x000fffffffffffffll) | 0x3ff0000000000000ll);
+    // round(256 / (1 + (i + 0.5) / 64)) = floor((32768 + (2 i + 129) / 2) / (2 i + 129)), no ties
+    const int d = 2 * i + 129, c256 = (32768 + (d >> 1)) / d;
+    const double r = fma(f, (double)c256 * 0.00390625, -1.0);
+    const float q = (float)r;
+    const float t = q * q * fmaf(q, fmaf(q, fmaf(q, fmaf(q, -1.0f / 6.0f, 0.2f), -0.25f), 1.0f / 3.0f), -0.5f);
+    return fma((double)e, 0.6931471805599453, sel_log_c[i]) + (r + (double)t);
 }
 
 struct SelP {
@@ -120,237 +184,321 @@ struct SelP {
     unsigned *token, *parent, *done_out;
 };
 
-__device__ void sel_part(const SelP &p, SelSmem &sm, const float *row, int first, int last, bool with_eos, SelPart *out) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x, nwarps = nthreads >> 5;
-    const SelRange r = sel_range(row, first, last);
-    float top = -INFINITY, sum = 0.0f, best = -INFINITY;
-    unsigned best_token = 0;
-    for (int v = tid; v < r.vecs; v += 4 * nthreads) {
-        float4 x[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int w = v + u * nthreads;
-            x[u] = w < r.vecs ? sel_load(r, w) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        }
-        float m = top;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            x[u].x = drop_nan(x[u].x); x[u].y = drop_nan(x[u].y);
-            x[u].z = drop_nan(x[u].z); x[u].w = drop_nan(x[u].w);
-            const float m4 = fmaxf(fmaxf(x[u].x, x[u].y), fmaxf(x[u].z, x[u].w));
-            if (m4 > best) {           // ascending tokens: equal logits keep the lower one
-                const unsigned t = (unsigned)(r.first - r.shift + 4 * (v + u * nthreads));
-                best = m4;
-                best_token = x[u].x == m4 ? t : x[u].y == m4 ? t + 1 : x[u].z == m4 ? t + 2 : t + 3;
-            }
-            m = fmaxf(m, m4);
-        }
-        if (m == -INFINITY) continue;
-        sum = __fmul_rn(sum, top == m ? 1.0f : sel_exp(top, m));
-        top = m;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            sum += (sel_exp(x[u].x, m) + sel_exp(x[u].y, m)) + (sel_exp(x[u].z, m) + sel_exp(x[u].w, m));
-    }
-    if (with_eos && tid == 0) {        // one token behind the range
-        const float x = drop_nan(row[p.eos]);
-        if (x > best) { best = x; best_token = (unsigned)p.eos; }
-        if (x != -INFINITY) {
-            const float m = fmaxf(top, x);
-            sum = __fmul_rn(sum, top == m ? 1.0f : sel_exp(top, m)) + sel_exp(x, m);
-            top = m;
-        }
-    }
-    const unsigned long long mine = best == -INFINITY ? 0ull : sel_key(best, best_token);
+__device__ __forceinline__ void copy_async(float4 *to, const float4 *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
 
-    // the part's maximum and sum, and the maxima of groups of eight threads
-    float wtop = warp_max(top);
-    double wsum = top == -INFINITY ? 0.0 : (double)sum * (double)(top == wtop ? 1.0f : sel_exp(top, wtop));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) wsum += __shfl_xor_sync(MB_FULL, wsum, o);
-    unsigned long long g = mine;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) g = max_u64(g, __shfl_xor_sync(MB_FULL, g, o));
-    if (lane == 0) { sm.wtop[warp] = wtop; sm.wsum[warp] = wsum; }
-    if ((lane & 7) == 0) sm.group[tid >> 3] = g;
-    if (tid == 0) sm.n_reach = 0;
-    __syncthreads();
+// Asks for the whole pieces of a range to be brought into L2, 64 KB at a time.
+__device__ __forceinline__ void prefetch_row(const SelRange &r) {
+    for (int v = r.whole_from; v < r.whole_to; v += 4096) {
+        const unsigned bytes = 16u * (unsigned)min(4096, r.whole_to - v);
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(r.base + v), "r"(bytes) : "memory");
+    }
+}
 
-    // the bound: the beams-th largest group maximum, 0 when fewer groups have one
-    const int groups = nthreads >> 3;
-    unsigned long long bound = 0;
+// Maximum and sum of exponentials of the tokens a thread has seen; NaN is passed over by the
+// maximum and shows in the sum.  `most` receives the pieces' maxima.
+template <int N>
+__device__ __forceinline__ void sel_take(const float4 (&x)[N], float (&most)[N], float &top, float &sum) {
+    float m = top;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int i = lane + 32 * half;
-        const unsigned long long k = i < groups ? sm.group[i] : 0ull;
-        int above = 0;
-        for (int j = 0; j < groups; ++j) above += sm.group[j] > k;
-        const unsigned hit = __ballot_sync(MB_FULL, k != 0ull && above == p.beams - 1);
-        if (hit) bound = __shfl_sync(MB_FULL, k, __ffs(hit) - 1);
+    for (int u = 0; u < N; ++u) {
+        most[u] = fmaxf(fmaxf(x[u].x, x[u].y), fmaxf(x[u].z, x[u].w));
+        m = fmaxf(m, most[u]);
     }
-    // tokens that reach it: the whole warp reads again what a thread with one has seen
-    unsigned todo = __ballot_sync(MB_FULL, mine != 0ull && mine >= bound);
-    while (todo) {
-        const int owner = __ffs(todo) - 1;
-        todo &= todo - 1;
-        for (int v = warp * 32 + owner + lane * nthreads; v < r.vecs; v += 32 * nthreads) {
-            const float4 x = sel_load(r, v);
-            const unsigned t = (unsigned)(r.first - r.shift + 4 * v);
-            const float e[4] = {drop_nan(x.x), drop_nan(x.y), drop_nan(x.z), drop_nan(x.w)};
+    if (m > top) { sum = __fmul_rn(sum, sel_exp(top, m)); top = m; }
+    const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (e[j] == -INFINITY) continue;
-                const unsigned long long k = sel_key(e[j], t + j);
-                if (k < bound) continue;
-                const unsigned at = atomicAdd(&sm.n_reach, 1u);
-                if (at < SEL_CAP) sm.reach[at] = k;
-            }
-        }
-        if (with_eos && warp == 0 && owner == 0 && lane == 0) {
-            const float x = drop_nan(row[p.eos]);
-            if (x != -INFINITY && sel_key(x, (unsigned)p.eos) >= bound) {
-                const unsigned at = atomicAdd(&sm.n_reach, 1u);
-                if (at < SEL_CAP) sm.reach[at] = sel_key(x, (unsigned)p.eos);
-            }
-        }
+    for (int u = 0; u < N; ++u)
+        sum += (sel_exp(x[u].x, ref) + sel_exp(x[u].y, ref)) + (sel_exp(x[u].z, ref) + sel_exp(x[u].w, ref));
+}
+
+// The keys of a piece's tokens that reach the bound into the list; `most`: the piece's maximum.
+__device__ __forceinline__ void sel_reach(SelScratch &w, const float4 &x, float most, unsigned token, float bound) {
+    if (!(most >= bound)) return;      // nearly every piece
+    const float e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (!(e[j] >= bound) || e[j] == -INFINITY) continue;
+        const unsigned at = atomicAdd(&w.n_reach, 1u);
+        if (at < SEL_CAP) w.reach[at] = sel_key(e[j], token + j);
     }
-    if (tid < MB_BEAM_MAX) out->key[tid] = 0ull;       // out may lie in another CTA's shared memory
+}
+
+// The bound of a part from the largest logit each thread has seen: the beams-th largest of 32
+// group maxima, -inf when fewer groups have seen a token.  All threads of the CTA.
+template <int NTHREADS>
+__device__ __forceinline__ float sel_bound(SelScratch &w, float top, int beams) {
+    constexpr int GROUP = NTHREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31;
+#pragma unroll
+    for (int o = GROUP >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(MB_FULL, top, o));
+    if (tid % GROUP == 0) w.group[tid / GROUP] = top;
     __syncthreads();
-    const unsigned n = sm.n_reach;
-    if (n <= SEL_CAP) {
-        // keys are distinct: a key's place is the number of larger ones
-        for (unsigned i = tid; i < n; i += nthreads) {
-            const unsigned long long k = sm.reach[i];
-            int above = 0;
-            for (unsigned j = 0; j < n; ++j) above += sm.reach[j] > k;
-            if (above < p.beams) out->key[above] = k;
+    if (tid < 32) {
+        const float mine = w.group[lane];
+        int reach = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) reach += w.group[j] >= mine;
+        // largest value that at least `beams` groups reach
+        const unsigned best = __reduce_max_sync(MB_FULL, reach >= beams ? sel_bits(mine) : 0u);
+        if (lane == 0) w.bound = sel_logit((unsigned long long)best << 32);
+    }
+    __syncthreads();
+    return w.bound;
+}
+
+// FIT: parts of at most SEL_HELD pieces per thread.
+template <bool FIT>
+__global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 : 1) k_beam_select(SelP p) {
+    __shared__ SelSmem sm;
+    extern __shared__ float4 ring[];
+    constexpr int NT = FIT ? SEL_FIT_THREADS : SEL_THREADS, WARPS = NT / 32;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_arrive();
+    mb_pdl_wait();
+    mb_pdl_trigger();
+    const int rank = (int)cluster.block_rank(), size = (int)cluster.num_blocks();
+    const int request = blockIdx.x / size;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, beams = p.beams, parts = p.parts;
+    const unsigned live = p.live != nullptr ? *p.live : 0xffffffffu;
+    // what the first CTA needs at the end is on its way from here on
+    const int n = beams * parts * beams, mine = tid < n ? tid / (parts * beams) : 0;
+    const float score = p.score[request * beams + mine];
+    const unsigned done = __ballot_sync(MB_FULL, p.done != nullptr && lane < beams && p.done[request * beams + lane] != 0);
+    const bool allow = p.has_eos && (p.allow_eos == nullptr || p.allow_eos[request] != 0);
+    if ((unsigned)request >= live) {   // the whole cluster
+        cluster.barrier_wait();
+        return;
+    }
+    if (tid < SEL_SHARE) sm.work[tid].n_reach = 0;
+
+    const int per = (p.codebook + parts - 1) / parts;
+    auto range = [&](int i) {          // of part i of the request
+        const int b = i / parts, from = min((i - b * parts) * per, p.codebook);
+        return sel_range(p.logits + (size_t)(request * beams + b) * p.logits_stride, from, min(from + per, p.codebook));
+    };
+    auto has = [&](int i) { return i < beams * parts && !(done >> (i / parts) & 1u); };
+    auto has_eos = [&](int i) { return allow && tid == 0 && (i + 1) % parts == 0; };
+
+    // this CTA's parts: rank, rank + size, ... of the request's
+    for (int i = rank, q = 0; i < beams * parts; i += size, ++q) {
+        if (!has(i)) continue;
+        SelScratch &w = sm.work[q];
+        const SelRange r = range(i);
+        if (!FIT && tid == 0 && has(i + size)) prefetch_row(range(i + size));
+        // what lies beside the whole pieces: a ragged first or last one, which falls to one thread,
+        // and the token behind the range
+        const int edge = tid == 0 && r.whole_from > 0 ? 0 : tid == NT - 1 && r.whole_to < r.vecs ? r.vecs - 1 : -1;
+        float4 beside[2] = {no_tokens(), no_tokens()};
+        if (edge >= 0) beside[0] = drop_nan(sel_load(r, edge));
+        if (has_eos(i)) beside[1].x = drop_nan(r.row[p.eos]);
+        const int whole = r.whole_to - r.whole_from;
+        const float4 *at = r.base + r.whole_from + tid;            // this thread's next piece
+        unsigned token = (unsigned)(r.origin + 4 * (r.whole_from + tid));
+        float4 x[SEL_HELD];
+        float most[SEL_HELD], beside_most[2], bound, top = -INFINITY, sum = 0.0f;
+        if (FIT) {
+#pragma unroll
+            for (int u = 0; u < SEL_HELD; ++u) {
+                x[u] = no_tokens();
+                if (tid + u * NT < whole) x[u] = at[u * NT];
+            }
+            sel_take(x, most, top, sum);
+            sel_take(beside, beside_most, top, sum);
+            bound = sel_bound<NT>(w, top, beams);
+#pragma unroll
+            for (int u = 0; u < SEL_HELD; ++u) sel_reach(w, x[u], most[u], token + 4 * u * NT, bound);
+        } else {
+            constexpr int TURN = SEL_HELD * NT;
+            const int turns = whole / TURN, rest = whole - turns * TURN;   // whole turns, pieces of the last one
+            const float4 *from = at;                                       // next piece to ask for
+            float4 *to = ring + tid;
+            auto ask = [&](int turn) {
+                if (turn < turns) {
+#pragma unroll
+                    for (int u = 0; u < SEL_HELD; ++u) copy_async(to + u * NT, from + u * NT);
+                } else if (turn == turns) {
+#pragma unroll
+                    for (int u = 0; u < SEL_HELD; ++u)
+                        if (tid + u * NT < rest) copy_async(to + u * NT, from + u * NT);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                from += TURN;
+                to = to == ring + (SEL_DEPTH - 1) * TURN + tid ? ring + tid : to + TURN;
+            };
+            for (int turn = 0; turn < SEL_DEPTH; ++turn) ask(turn);
+            sel_take(beside, beside_most, top, sum);
+            for (int turn = 0; turn <= turns; ++turn, token += 4 * TURN) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(SEL_DEPTH - 1) : "memory");
+#pragma unroll
+                for (int u = 0; u < SEL_HELD; ++u) x[u] = to[u * NT];      // the place asked for next
+                if (turn == turns)
+#pragma unroll
+                    for (int u = 0; u < SEL_HELD; ++u)
+                        if (tid + u * NT >= rest) x[u] = no_tokens();
+                ask(turn + SEL_DEPTH);
+                sel_take(x, most, top, sum);
+                if ((turn & (turn + 1)) == 0) bound = sel_bound<NT>(w, top, beams);
+#pragma unroll
+                for (int u = 0; u < SEL_HELD; ++u) sel_reach(w, x[u], most[u], token + 4 * u * NT, bound);
+            }
         }
-    } else {
-        // Many tokens reach the bound (their large logits lie in a few threads' pieces): take
-        // the largest key below the last one, once per place, from a fresh pass each.
+        sel_reach(w, beside[0], beside_most[0], (unsigned)(r.origin + 4 * edge), bound);
+        sel_reach(w, beside[1], beside_most[1], (unsigned)p.eos, bound);
+        if (sum != sum) {              // NaN among the logits, or +inf: the sum again without them
+            sum = 0.0f;
+            top = -INFINITY;
+            for (int v = tid; v < whole; v += NT, at += NT) {
+                const float4 y[1] = {drop_nan(*at)};
+                float unused[1];
+                sel_take(y, unused, top, sum);
+            }
+            sel_take(beside, beside_most, top, sum);
+        }
+        const float wtop = warp_max(top);
+        double wsum = top == -INFINITY ? 0.0 : (double)__fmul_rn(sum, top == wtop ? 1.0f : sel_exp(top, wtop));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) wsum += __shfl_xor_sync(MB_FULL, wsum, o);
+        if (lane == 0) { w.wtop[warp] = wtop; w.wsum[warp] = wsum; }
+    }
+    __syncthreads();
+    cluster.barrier_wait();            // the first CTA has started: its memory may be written
+    SelPart *found = cluster.map_shared_rank(sm.part, 0);
+    for (int i = rank, q = 0; i < beams * parts; i += size, ++q) {
+        if (!has(i)) continue;
+        SelScratch &w = sm.work[q];
+        SelPart *out = &found[i];
+        if (warp == WARPS - 1 - q) {   // the sum of the part
+            const float t = lane < WARPS ? w.wtop[lane] : -INFINITY;
+            const float m = warp_max(t);
+            double all = t == -INFINITY ? 0.0 : w.wsum[lane] * (double)(t == m ? 1.0f : sel_exp(t, m));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(MB_FULL, all, o);
+            if (lane == 0) {
+                out->top = m;
+                out->sum = all;
+                // the largest term is 1, unless +inf is among the logits or there is no token: no distribution
+                if (parts == 1) out->lse = all >= 0.5 ? (double)m + sel_log(all) : (double)NAN;
+            }
+        }
+        const int reach = (int)w.n_reach;
+        if (reach <= SEL_CAP) {
+            // keys are distinct: a key's place is the number of larger ones; four threads share one
+            for (int j0 = 0; j0 < reach; j0 += NT / 4) {
+                const int j = j0 + (tid >> 2);
+                const unsigned long long k = j < reach ? w.reach[j] : 0ull;
+                int above = 0;
+#pragma unroll 4
+                for (int o = tid & 3; o < reach; o += 4) above += w.reach[o] > k;
+                above += __shfl_xor_sync(MB_FULL, above, 1);
+                above += __shfl_xor_sync(MB_FULL, above, 2);
+                if (j < reach && above < beams && (tid & 3) == 0) out->key[above] = k;
+            }
+            if (tid >= reach && tid < beams) out->key[tid] = 0ull;
+            continue;
+        }
+        // the largest key below the last one, once per place
+        const SelRange r = range(i);
+        const unsigned long long eos_key = has_eos(i) && drop_nan(r.row[p.eos]) > -INFINITY
+                                               ? sel_key(r.row[p.eos], (unsigned)p.eos) : 0ull;
         unsigned long long last_key = ~0ull;
-        for (int place = 0; place < p.beams; ++place) {
-            unsigned long long k = 0;
-            for (int v = tid; v < r.vecs; v += nthreads) {
+        for (int place = 0; place < beams; ++place) {
+            unsigned long long k = eos_key < last_key ? eos_key : 0ull;
+            for (int v = tid; v < r.vecs; v += NT) {
                 const float4 x = sel_load(r, v);
-                const unsigned t = (unsigned)(r.first - r.shift + 4 * v);
-                const float e[4] = {drop_nan(x.x), drop_nan(x.y), drop_nan(x.z), drop_nan(x.w)};
+                const unsigned t = (unsigned)(r.origin + 4 * v);
+                const float e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (e[j] == -INFINITY) continue;
+                    if (!(e[j] > -INFINITY)) continue;
                     const unsigned long long c = sel_key(e[j], t + j);
                     if (c < last_key) k = max_u64(k, c);
                 }
             }
-            if (with_eos && tid == 0) {
-                const float x = drop_nan(row[p.eos]);
-                const unsigned long long c = x == -INFINITY ? 0ull : sel_key(x, (unsigned)p.eos);
-                if (c < last_key) k = max_u64(k, c);
-            }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) k = max_u64(k, __shfl_xor_sync(MB_FULL, k, o));
             __syncthreads();
-            if (lane == 0) sm.wkey[warp] = k;
+            if (lane == 0) w.wkey[warp] = k;
             __syncthreads();
             k = 0;
-            for (int w = 0; w < nwarps; ++w) k = max_u64(k, sm.wkey[w]);
+            for (int v = 0; v < WARPS; ++v) k = max_u64(k, w.wkey[v]);
             if (tid == 0) out->key[place] = k;
-            last_key = k;
-            if (k == 0ull) break;
+            last_key = k;              // more than SEL_CAP keys: never 0
         }
-    }
-    if (tid == 0) {
-        float m = -INFINITY;
-        for (int w = 0; w < nwarps; ++w) m = fmaxf(m, sm.wtop[w]);
-        double s = 0.0;
-        for (int w = 0; w < nwarps; ++w)
-            if (sm.wtop[w] != -INFINITY) s += sm.wsum[w] * exp((double)sm.wtop[w] - (double)m);
-        out->top = m;
-        out->sum = s;
-    }
-    __syncthreads();                   // sm is used again by the next part
-}
-
-__global__ void __launch_bounds__(512) k_beam_select(SelP p) {
-    __shared__ SelSmem sm;
-    mb_pdl_wait();
-    mb_pdl_trigger();
-    cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), size = (int)cluster.num_blocks();
-    const int request = blockIdx.x / size;
-    if (p.live != nullptr && (unsigned)request >= *p.live) return;      // the whole cluster
-    const int tid = threadIdx.x, beams = p.beams, parts = p.parts;
-    SelSmem *first = cluster.map_shared_rank(&sm, 0);
-    cluster.sync();                    // the first CTA's memory may be written from here on
-    const bool allow = p.has_eos && (p.allow_eos == nullptr || p.allow_eos[request] != 0);
-    for (int i = rank; i < beams * parts; i += size) {
-        const int b = i / parts, part = i - b * parts;
-        const int row = request * beams + b;
-        if (p.done != nullptr && p.done[row] != 0) continue;
-        const int per = (p.codebook + parts - 1) / parts;
-        const int from = min(part * per, p.codebook), to = min(from + per, p.codebook);
-        sel_part(p, sm, p.logits + (size_t)row * p.logits_stride, from, to, allow && part == parts - 1, &first->part[i]);
     }
     cluster.sync();
     if (rank != 0) return;
 
-    if (tid < beams) {
-        const bool done = p.done != nullptr && p.done[request * beams + tid] != 0;
-        double lse = 0.0;
-        if (done) {
-            for (int j = 0; j < parts; ++j)
-                for (int k = 0; k < beams; ++k) sm.part[tid * parts + j].key[k] = j + k == 0 ? sel_key(0.0f, (unsigned)p.eos) : 0ull;
+    // the continuations of all parts, at most 16 x 16, and their scores as ordered integers
+    if (tid < beams && parts > 1 && !(done >> tid & 1u)) {
+        SelPart *of = sm.part + tid * parts;
+        float m = -INFINITY;
+        for (int j = 0; j < parts; ++j) m = fmaxf(m, of[j].top);
+        double all = 0.0;
+        for (int j = 0; j < parts; ++j)
+            if (of[j].top != -INFINITY) all += of[j].sum * (double)(of[j].top == m ? 1.0f : sel_exp(of[j].top, m));
+        of[0].lse = all >= 0.5 ? (double)m + sel_log(all) : (double)NAN;
+    }
+    if (parts > 1) __syncthreads();
+    if (tid < beams * parts) sm.order[tid * SEL_PAD + beams] = 0ull;
+    if (tid < n) {
+        const int part = tid / beams, k = tid - part * beams, b = mine, to = part * SEL_PAD + k;
+        unsigned long long key;
+        double c;
+        if (done >> b & 1u) {
+            key = part == b * parts && k == 0 ? sel_key(0.0f, (unsigned)p.eos) : 0ull;
+            c = score;
         } else {
-            float m = -INFINITY;
-            for (int j = 0; j < parts; ++j) m = fmaxf(m, sm.part[tid * parts + j].top);
-            double s = 0.0;
-            for (int j = 0; j < parts; ++j)
-                if (sm.part[tid * parts + j].top != -INFINITY)
-                    s += sm.part[tid * parts + j].sum * exp((double)sm.part[tid * parts + j].top - (double)m);
-            lse = (double)m + log(s);
+            key = sm.part[part].key[k];
+            c = (double)score + ((double)sel_logit(key) - sm.part[b * parts].lse);
         }
-        sm.lse[tid] = lse;
+        sm.key[to] = key;
+        sm.score[to] = c;
+        const long long bits = __double_as_longlong(c + 0.0);
+        // 0: no candidate (NaN and -inf among them)
+        sm.order[to] = key != 0ull && c > -INFINITY ? (unsigned long long)(bits < 0 ? ~bits : bits | (1ll << 63)) : 0ull;
     }
     __syncthreads();
-    // ranked continuations: place (part, k) of the list; at most 16 x 16
-    const int n = beams * parts * beams;
-    for (int i = tid; i < n; i += blockDim.x) {
-        const int part = i / beams, b = part / parts;
-        const unsigned long long key = sm.part[part].key[i - part * beams];
-        const double c = (double)p.score[request * beams + b] + ((double)sel_logit(key) - sm.lse[b]);
-        sm.score[i] = key != 0ull && c > -INFINITY ? c : -INFINITY;     // NaN is no candidate
-    }
-    __syncthreads();
-    int taken = 0;
-    for (int i = tid; i < n; i += blockDim.x) {
-        const int part = i / beams, b = part / parts;
-        const unsigned long long key = sm.part[part].key[i - part * beams];
-        const double c = sm.score[i];
-        if (c == -INFINITY) continue;
-        int above = 0;
-        for (int j = 0; j < n; ++j) {
-            const int q = j / beams, o = q / parts;
-            const double d = sm.score[j];
-            above += d > c || (d == c && (o < b || (o == b && sm.part[q].key[j - q * beams] > key)));
+    // The lists fall, so the best continuation left is the best of their heads: one warp takes
+    // `beams` of them, a list per lane.
+    if (tid >= 32) return;
+    const int lists = beams * parts, last = tid * SEL_PAD + beams;     // behind a list lies a 0
+    int at = tid * SEL_PAD, found_all = 0;
+    unsigned long long head = tid < lists ? sm.order[at] : 0ull, next = tid < lists ? sm.order[at + 1] : 0ull;
+    for (; found_all < beams; ++found_all) {
+        const unsigned high = __reduce_max_sync(MB_FULL, (unsigned)(head >> 32));
+        if (high == 0u) break;                         // nothing is left (an order's first bits are not 0)
+        unsigned best = __ballot_sync(MB_FULL, (unsigned)(head >> 32) == high);
+        if (best & (best - 1)) {
+            const bool first = (unsigned)(head >> 32) == high;
+            const unsigned low = __reduce_max_sync(MB_FULL, first ? (unsigned)head : 0u);
+            best = __ballot_sync(MB_FULL, first && (unsigned)head == low);
+            // equal scores: the lower beam, which is the lower list; parts of one beam by their keys
+            int winner = __ffs(best) - 1;
+            for (unsigned more = best & (best - 1); parts > 1 && more != 0u; more &= more - 1) {
+                const int other = __ffs(more) - 1;
+                const unsigned long long a = sm.key[__shfl_sync(MB_FULL, at, winner)], o = sm.key[__shfl_sync(MB_FULL, at, other)];
+                if (other / parts == winner / parts && o > a) winner = other;
+            }
+            best = 1u << winner;
         }
-        if (above >= beams) continue;
-        const int at = request * beams + above;
-        const unsigned t = sel_token(key);
-        p.score_out[at] = (float)c;
-        p.token[at] = t;
-        p.parent[at] = (unsigned)b;
-        if (p.done_out != nullptr) p.done_out[at] = t == (unsigned)p.eos ? 1u : 0u;
-        ++taken;
+        const bool won = best >> tid & 1u;
+        if (won) sm.taken[found_all] = at;
+        head = won ? next : head;
+        at += won;
+        next = sm.order[tid < lists ? min(at + 1, last) : 0];
     }
-    // places without a continuation: a dead beam that stays where it is
-    taken = __syncthreads_count(taken > 0) ;
-    if (tid >= taken && tid < beams) {
-        const int at = request * beams + tid;
-        p.score_out[at] = -INFINITY;
-        p.token[at] = 0u;
-        p.parent[at] = (unsigned)tid;
-        if (p.done_out != nullptr) p.done_out[at] = 0u;
-    }
+    __syncwarp();
+    if (tid >= beams) return;
+    const int to = request * beams + tid;
+    const bool alive = tid < found_all;
+    const int from = alive ? sm.taken[tid] : 0;
+    const unsigned t = alive ? sel_token(sm.key[from]) : 0u;
+    p.score_out[to] = alive ? (float)sm.score[from] : -INFINITY;
+    p.token[to] = t;
+    p.parent[to] = alive ? (unsigned)(from / SEL_PAD / parts) : (unsigned)tid;         // dead: stays where it is
+    if (p.done_out != nullptr) p.done_out[to] = alive && t == (unsigned)p.eos ? 1u : 0u;
 }
 
 // ------------------------------------------------------------------------ reordering
@@ -431,6 +579,44 @@ __global__ void __launch_bounds__(256) k_beam_reorder(ReorderP p) {
 
 }  // namespace
 
+namespace {
+
+int sel_launch(void (*kernel)(SelP), const SelP &p, size_t requests, int size, int threads, unsigned smem, cudaStream_t stream,
+               int *resident) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(requests * (size_t)size));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = mb_pdl_enabled() ? 2u : 1u;
+    if (resident != nullptr) {         // clusters of this size that the device holds at once
+        cfg.numAttrs = 1u;
+        return (int)cudaOccupancyMaxActiveClusters(resident, kernel, &cfg);
+    }
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+}  // namespace
+
+extern "C" int mb_beam_init(int *clusters) {
+    const int rc = (int)cudaFuncSetAttribute(k_beam_select<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_RING_BYTES);
+    SelP none = {};
+    for (int size = 1; rc == 0 && size <= SEL_CLUSTER; ++size) {
+        const int q = sel_launch(k_beam_select<false>, none, 1, size, SEL_THREADS, SEL_RING_BYTES, 0, &clusters[size]);
+        if (q != 0) return q;
+        if (clusters[size] < 1) clusters[size] = 1;
+    }
+    return rc;
+}
+
 extern "C" int mb_beam_select(const mb_beam_select_args *a, mb_stream stream) {
     SelP p;
     p.logits = a->logits;
@@ -453,23 +639,23 @@ extern "C" int mb_beam_select(const mb_beam_select_args *a, mb_stream stream) {
     p.parts = 1;
     while (p.beams * p.parts * 2 <= SEL_CLUSTER && p.codebook / (2 * p.parts) >= 2048) p.parts *= 2;
     const int pieces = p.beams * p.parts;
-    const int rounds = (pieces + SEL_CLUSTER - 1) / SEL_CLUSTER;
-    const int size = (pieces + rounds - 1) / rounds;
-    const int threads = p.codebook / p.parts >= 8192 ? 512 : 256;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a->requests * (size_t)size));
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)size;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = mb_pdl_enabled() ? 2u : 1u;
-    return (int)cudaLaunchKernelEx(&cfg, k_beam_select, p);
+    // a part of at most 16 tokens per thread stays in registers: small CTAs, as many as there are
+    if ((p.codebook + p.parts - 1) / p.parts <= 4 * SEL_HELD * SEL_FIT_THREADS) {
+        const int rounds = (pieces + SEL_CLUSTER - 1) / SEL_CLUSTER, size = (pieces + rounds - 1) / rounds;
+        return sel_launch(k_beam_select<true>, p, a->requests, size, SEL_FIT_THREADS, 0u, (cudaStream_t)stream, nullptr);
+    }
+    // long parts: the cluster size with the fewest parts one after the other, counting the waves
+    // that the device needs for all clusters (24 requests of 16 beams: 6 CTAs, all at once, and
+    // three parts each; 8 CTAs take two waves of two)
+    int best = 0, least = 0;
+    for (int size = SEL_CLUSTER; size >= 1; --size) {
+        const int share = (pieces + size - 1) / size;
+        if (share > SEL_SHARE || size > pieces) continue;
+        const size_t waves = (a->requests + (size_t)a->clusters[size] - 1u) / (size_t)a->clusters[size];
+        const int cost = (int)(waves > 1000000u ? 1000000u : waves) * share;
+        if (best == 0 || cost < least) { best = size; least = cost; }
+    }
+    return sel_launch(k_beam_select<false>, p, a->requests, best, SEL_THREADS, SEL_RING_BYTES, (cudaStream_t)stream, nullptr);
 }
 
 extern "C" int mb_beam_reorder(const mb_beam_reorder_args *a, mb_stream stream) {

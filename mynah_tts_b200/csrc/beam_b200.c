@@ -168,6 +168,7 @@ int mynah_b200_beam_select(void *state, const mynah_b200_beam_select_args *a, ch
     m.token = a->dev_token;
     m.parent = a->dev_parent;
     m.done_out = a->dev_done_out;
+    m.clusters = st->beam_clusters;
     device_scope scope;
     if (enter_device(st, &scope, error, cap) != 0) return -1;
     const int rc = mb_cuda(mb_beam_select(&m, st->stream), "beam selection", error, cap);

@@ -101,20 +101,19 @@ __device__ __forceinline__ unsigned own_row(const LaneP &p, const LaneView &w, u
 }
 
 template <typename T>
-struct Piece;                      // 16 bytes of a row as floats
+struct Piece;                      // 16 bytes of a row: their elements as floats
 template <>
 struct Piece<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void get(const float *at, float (&x)[4]) {
-        const float4 v = *reinterpret_cast<const float4 *>(at);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    static __device__ __forceinline__ void get(const uint4 &v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y);
+        x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
     }
 };
 template <>
 struct Piece<__half> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void get(const __half *at, float (&x)[8]) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(at);
+    static __device__ __forceinline__ void get(const uint4 &v, float (&x)[8]) {
         const unsigned u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -136,7 +135,23 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
     __shared__ unsigned warp_sum_s[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = (blockDim.x + 31) >> 5;
     unsigned carry = 0;
-    for (int b0 = 0; b0 < p.lanes; b0 += blockDim.x) {
+    if (p.lanes <= 32) {               // one warp, one barrier
+        if (warp == 0) {
+            unsigned n = 0;
+            if (lane < p.lanes) {
+                const LaneView w = lane_view(p, lane);
+                n = w.prefix_rows + w.own_rows;
+            }
+            unsigned x = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(MB_FULL, x, o);
+                if (lane >= o) x += y;
+            }
+            if (lane < p.lanes) off[lane] = x - n;
+            carry = __shfl_sync(MB_FULL, x, 31);
+        }
+    } else for (int b0 = 0; b0 < p.lanes; b0 += blockDim.x) {
         const int b = b0 + tid;
         unsigned n = 0;
         if (b < p.lanes) {
@@ -169,38 +184,47 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
 }
 
 // LPR lanes of a warp share a row's head (16 elements each), so a warp takes 32 / LPR rows at
-// a time; a row's score is complete in its lanes after log2(LPR) exchanges, and every group of
-// LPR lanes keeps its own running maximum and sum, joined once per run.
-template <typename T, int LPR>
+// a time, U times over before it uses them; a row's score is complete in its lanes after
+// log2(LPR) exchanges, and every group of LPR lanes keeps its own running maximum and sum,
+// joined once per run.  Few heads: `phases` warps share a head's rows and join through shared
+// memory.
+template <typename T, int LPR, int U>
 __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP p) {
     extern __shared__ unsigned sm_off[];
     __shared__ unsigned s_run;
+    __shared__ float s_acc[WARPS_MAX][MB_LANE_HEAD_WIDTH_MAX];
+    __shared__ float2 s_stat[WARPS_MAX];
     constexpr int PER = Piece<T>::N, V = 16 / PER, GROUPS = 32 / LPR;
     mb_pdl_wait();
     mb_pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int step = GROUPS * p.phases;
-    lane_schedule(p, sm_off, &s_run, gridDim.x, step);
+    const int step = GROUPS * U * p.phases;
+    lane_schedule(p, sm_off, &s_run, gridDim.x, GROUPS * p.phases);
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         for (int i = threadIdx.x; i <= p.lanes; i += blockDim.x) p.offset[i] = sm_off[i];
         if (threadIdx.x == 0) p.offset[p.lanes + 1] = s_run;
     }
-    const int head = blockIdx.y * p.heads_per_cta + warp % p.heads_per_cta, phase = warp / p.heads_per_cta;
+    // a warp without a head (the last CTA row's) works on the last one and stores nothing
+    const int wanted = blockIdx.y * p.heads_per_cta + warp % p.heads_per_cta, phase = warp / p.heads_per_cta;
+    const int head = min(wanted, p.heads - 1);
     const unsigned total = sm_off[p.lanes], run = s_run;
-    unsigned long long begin = (unsigned long long)blockIdx.x * run;
-    if (begin >= total || head >= p.heads) return;
+    const unsigned long long begin = (unsigned long long)blockIdx.x * run;
+    if (begin >= total) return;
     const unsigned end = (unsigned)min((unsigned long long)total, begin + run);
     unsigned at = (unsigned)begin;
     int b = 0;                                   // the lane that row `at` belongs to
-    for (int lo = 0, hi = p.lanes; lo < hi;) {
+    for (int lo = 0, hi = p.lanes - 1; lo < hi;) {
         const int mid = (lo + hi + 1) >> 1;
-        if (mid < p.lanes && sm_off[mid] <= at) { lo = mid; b = mid; } else hi = mid - 1;
+        if (sm_off[mid] <= at) lo = b = mid; else hi = mid - 1;
     }
-    while (sm_off[b + 1] <= at) ++b;
     const int group = lane / LPR, part = lane % LPR;
     while (at < end) {
         const LaneView w = lane_view(p, b);
         const unsigned first = at - sm_off[b], last = min(end, sm_off[b + 1]) - sm_off[b];
+        const T *pk = reinterpret_cast<const T *>(p.prefix_k) + w.prefix * p.prefix_stride + head * p.head_width;
+        const T *pv = reinterpret_cast<const T *>(p.prefix_v) + w.prefix * p.prefix_stride + head * p.head_width;
+        const T *ok = reinterpret_cast<const T *>(p.k) + w.slot * p.slot_stride + head * p.head_width;
+        const T *ov = reinterpret_cast<const T *>(p.v) + w.slot * p.slot_stride + head * p.head_width;
         float q[16], acc[16], top = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -208,15 +232,14 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
             q[i] = d < p.head_width ? p.qkv[(size_t)b * p.qkv_stride + head * p.head_width + d] * p.scale_log2 : 0.0f;
             acc[i] = 0.0f;
         }
-        const T *pk = reinterpret_cast<const T *>(p.prefix_k) + w.prefix * p.prefix_stride + head * p.head_width;
-        const T *pv = reinterpret_cast<const T *>(p.prefix_v) + w.prefix * p.prefix_stride + head * p.head_width;
-        const T *ok = reinterpret_cast<const T *>(p.k) + w.slot * p.slot_stride + head * p.head_width;
-        const T *ov = reinterpret_cast<const T *>(p.v) + w.slot * p.slot_stride + head * p.head_width;
         for (unsigned r0 = first + phase * GROUPS; r0 < last; r0 += step) {
-            const unsigned r = r0 + group;
-            const bool in = r < last;
-            const T *rk = ok, *rv = ov;
-            if (in) {
+            uint4 kx[U][V], vx[U][V];
+            bool in[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const unsigned r = r0 + u * GROUPS * p.phases + group;
+                in[u] = r < last;
+                const T *rk = ok, *rv = ov;
                 if (r < w.prefix_rows) {
                     const size_t o = (size_t)(r < w.prefix_head ? r : r + w.prefix_jump) * p.prefix_row_stride;
                     rk = pk + o;
@@ -226,39 +249,52 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
                     rk = ok + o;
                     rv = ov + o;
                 }
-            }
-            float kx[V][PER], vx[V][PER];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int d = (j * LPR + part) * PER;
-                if (in && d < p.head_width) {
-                    Piece<T>::get(rk + d, kx[j]);
-                    Piece<T>::get(rv + d, vx[j]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < PER; ++i) kx[j][i] = vx[j][i] = 0.0f;
+                for (int j = 0; j < V; ++j) {
+                    const int d = (j * LPR + part) * PER;
+                    kx[u][j] = vx[u][j] = make_uint4(0, 0, 0, 0);
+                    if (in[u] && d < p.head_width) {
+                        kx[u][j] = __ldg(reinterpret_cast<const uint4 *>(rk + d));
+                        vx[u][j] = __ldg(reinterpret_cast<const uint4 *>(rv + d));
+                    }
                 }
             }
-            float x = 0.0f;
+            float x[U], m = top;
 #pragma unroll
-            for (int j = 0; j < V; ++j)
+            for (int u = 0; u < U; ++u) {
+                x[u] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) x = fmaf(q[j * PER + i], kx[j][i], x);
+                for (int j = 0; j < V; ++j) {
+                    float k[PER];
+                    Piece<T>::get(kx[u][j], k);
 #pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) x += __shfl_xor_sync(MB_FULL, x, o);
-            if (!in) x = -INFINITY;
-            const float m = fmaxf(top, x);
+                    for (int i = 0; i < PER; ++i) x[u] = fmaf(q[j * PER + i], k[i], x[u]);
+                }
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) x[u] += __shfl_xor_sync(MB_FULL, x[u], o);
+                if (!in[u]) x[u] = -INFINITY;
+                m = fmaxf(m, x[u]);
+            }
             const float ref = m == -INFINITY ? 0.0f : m;      // nothing but -inf so far: weights 0, not NaN
-            const float keep = pow2(top - ref), e = pow2(x - ref);
+            const float keep = pow2(top - ref);
             top = m;
-            sum = fmaf(sum, keep, e);
+            sum *= keep;
 #pragma unroll
-            for (int j = 0; j < V; ++j)
+            for (int i = 0; i < 16; ++i) acc[i] *= keep;
 #pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    acc[j * PER + i] = fmaf(acc[j * PER + i], keep, in ? e * vx[j][i] : 0.0f);
+            for (int u = 0; u < U; ++u) {
+                const float e = pow2(x[u] - ref);
+                sum += e;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float v[PER];
+                    Piece<T>::get(vx[u][j], v);
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) acc[j * PER + i] = fmaf(e, v[i], acc[j * PER + i]);
+                }
+            }
         }
-        // join the groups of the warp
+        // join the groups of the warp, then its phases
         float m = top;
 #pragma unroll
         for (int o = LPR; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(MB_FULL, m, o));
@@ -266,7 +302,6 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
         sum *= f;
 #pragma unroll
         for (int o = LPR; o < 32; o <<= 1) sum += __shfl_xor_sync(MB_FULL, sum, o);
-        const size_t slot = ((size_t)(blockIdx.x + b) * p.phases + phase) * p.heads + head;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float a = acc[i] * f;
@@ -274,7 +309,35 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
             for (int o = LPR; o < 32; o <<= 1) a += __shfl_xor_sync(MB_FULL, a, o);
             acc[i] = a;
         }
-        if (group == 0) {
+        if (p.phases > 1) {
+            if (group == 0) {
+                if (part == 0) s_stat[warp] = make_float2(m, sum);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s_acc[warp][((i / PER) * LPR + part) * PER + i % PER] = acc[i];
+            }
+            __syncthreads();
+            if (phase == 0) {
+                float all = m;
+                for (int o = 1; o < p.phases; ++o) all = fmaxf(all, s_stat[warp + o * p.heads_per_cta].x);
+                const float ref = all == -INFINITY ? 0.0f : all;
+                const float g = pow2(m - ref);
+                sum *= g;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i] *= g;
+                for (int o = 1; o < p.phases; ++o) {
+                    const int other = warp + o * p.heads_per_cta;
+                    const float h = pow2(s_stat[other].x - ref);
+                    sum = fmaf(s_stat[other].y, h, sum);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        acc[i] = fmaf(s_acc[other][((i / PER) * LPR + part) * PER + i % PER], h, acc[i]);
+                }
+                m = all;
+            }
+            __syncthreads();
+        }
+        if (group == 0 && phase == 0 && wanted < p.heads) {
+            const size_t slot = (size_t)(blockIdx.x + b) * p.heads + head;
             if (part == 0) p.stat[slot] = make_float2(m, sum);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -292,68 +355,119 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
     }
 }
 
-// One warp per head of a lane: the new row's score, the lane's partials in row order, the
-// result, and the new row into the cache.  A lane whose cache is full or whose slot does not
-// exist is left out and sets the status word.
+// One CTA per head of a lane: the new row's score, the lane's partials, the result, and the new
+// row into the cache.  Four columns per thread, threads of the same columns take every
+// SLICES-th partial, MERGE_U at a time (a lane alone has hundreds).  A lane whose cache is full
+// or whose slot does not exist is left out and sets the status word.
+constexpr int MERGE_U = 4;
+
 template <typename T>
-__global__ void k_lane_merge(LaneP p) {
-    mb_pdl_wait();
-    mb_pdl_trigger();
-    const int b = blockIdx.x, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+__global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
+    __shared__ float4 s_acc[16][32];
+    __shared__ float2 s_stat[16];
+    const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // lane state and rows were written before k_lane_rows began
     if (p.live != nullptr && (unsigned)b >= *p.live) return;
     const LaneView w = lane_view(p, b);
+    const int column = tid % columns, slice = tid / columns, slices = blockDim.x / columns;
+    const int d = column * 4;
+    const bool mine = d < p.head_width;
+    const float *row = p.qkv + (size_t)b * p.qkv_stride + head * p.head_width + d;
+    T kt[4], vt[4];
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        kt[i] = (T)(mine ? row[p.width + i] : 0.0f);
+        vt[i] = (T)(mine ? row[2 * p.width + i] : 0.0f);
+        x = fmaf(mine ? row[i] * p.scale_log2 : 0.0f, (float)kt[i], x);
+    }
+    for (int o = columns >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(MB_FULL, x, o);
+    mb_pdl_wait();
+    mb_pdl_trigger();
     if (!w.ok) {
-        if (threadIdx.x == 0) atomicOr(p.status, 32);
+        if (tid == 0 && head == 0) atomicOr(p.status, 32);
         return;
     }
     const unsigned first = p.offset[b], last = p.offset[b + 1], run = p.offset[p.lanes + 1];
-    const unsigned part0 = last > first ? first / run : 0u, parts = last > first ? (last - 1) / run - part0 + 1 : 0u;
-    const int n = (int)parts * p.phases;
-    const size_t base = ((size_t)part0 + b) * p.phases;
-    const int d = lane * 4;
-    const bool mine = d < p.head_width;
-    for (int head = blockIdx.y * warps + (threadIdx.x >> 5); head < p.heads; head += gridDim.y * warps) {
-        const float *row = p.qkv + (size_t)b * p.qkv_stride + head * p.head_width + d;
-        float q[4] = {0, 0, 0, 0}, k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0}, acc[4];
-        if (mine)
+    const unsigned part0 = last > first ? first / run : 0u;
+    const int n = last > first ? (int)((last - 1) / run - part0) + 1 : 0;
+    const size_t base = (size_t)(part0 + b) * p.heads + head;
+    if (slice == 0 && mine) {
+        const size_t o = w.slot * p.slot_stride + (size_t)w.append * p.row_stride + head * p.head_width + d;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                q[i] = row[i] * p.scale_log2;
-                const T kt = (T)row[p.width + i], vt = (T)row[2 * p.width + i];
-                k[i] = (float)kt;
-                v[i] = (float)vt;
-                const size_t o = w.slot * p.slot_stride + (size_t)w.append * p.row_stride + head * p.head_width + d + i;
-                reinterpret_cast<T *>(p.k)[o] = kt;
-                reinterpret_cast<T *>(p.v)[o] = vt;
-            }
-        float x = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            reinterpret_cast<T *>(p.k)[o + i] = kt[i];
+            reinterpret_cast<T *>(p.v)[o + i] = vt[i];
+        }
+    }
+    // the first slice begins with the new row, the others with nothing
+    float top = slice == 0 ? x : -INFINITY, sum = slice == 0 ? 1.0f : 0.0f;
+    float4 acc = slice == 0 ? make_float4((float)vt[0], (float)vt[1], (float)vt[2], (float)vt[3]) : make_float4(0, 0, 0, 0);
+    if (slice == 0 && x == -INFINITY) { sum = 0.0f; acc = make_float4(0, 0, 0, 0); }
+    for (int i0 = slice; i0 < n; i0 += MERGE_U * slices) {
+        float2 s[MERGE_U];
+        float4 a[MERGE_U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x = fmaf(q[i], k[i], x);
-        x = warp_sum(x);
-        float top = x;
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, p.stat[(base + i) * p.heads + head].x);
-        top = warp_max(top);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        const float e = pow2(x - ref);
-        float sum = e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = e * v[i];
-        for (int i = 0; i < n; ++i) {
-            const float2 s = p.stat[(base + i) * p.heads + head];
-            const float f = pow2(s.x - ref);
-            sum = fmaf(s.y, f, sum);
-            if (mine) {
-                const float4 a = *reinterpret_cast<const float4 *>(p.acc + ((base + i) * p.heads + head) * p.head_width + d);
-                acc[0] = fmaf(a.x, f, acc[0]);
-                acc[1] = fmaf(a.y, f, acc[1]);
-                acc[2] = fmaf(a.z, f, acc[2]);
-                acc[3] = fmaf(a.w, f, acc[3]);
+        for (int u = 0; u < MERGE_U; ++u) {
+            const int i = i0 + u * slices;
+            s[u] = make_float2(-INFINITY, 0.0f);
+            a[u] = make_float4(0, 0, 0, 0);
+            if (i < n) {
+                const size_t at = base + (size_t)i * p.heads;
+                s[u] = p.stat[at];
+                if (mine) a[u] = *reinterpret_cast<const float4 *>(p.acc + at * p.head_width + d);
             }
         }
-        if (mine)
+        float m = top;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p.out[(size_t)b * p.out_stride + head * p.head_width + d + i] = __fdiv_rn(acc[i], sum);
+        for (int u = 0; u < MERGE_U; ++u) m = fmaxf(m, s[u].x);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        const float keep = pow2(top - ref);
+        top = m;
+        sum *= keep;
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+        for (int u = 0; u < MERGE_U; ++u) {
+            const float f = pow2(s[u].x - ref);
+            sum = fmaf(s[u].y, f, sum);
+            acc.x = fmaf(a[u].x, f, acc.x); acc.y = fmaf(a[u].y, f, acc.y);
+            acc.z = fmaf(a[u].z, f, acc.z); acc.w = fmaf(a[u].w, f, acc.w);
+        }
     }
+    // slices of the warp, then of the other warps
+    float m = top;
+    for (int o = columns; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(MB_FULL, m, o));
+    const float f = pow2(top - (m == -INFINITY ? 0.0f : m));
+    sum *= f;
+    acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+    for (int o = columns; o < 32; o <<= 1) {
+        sum += __shfl_xor_sync(MB_FULL, sum, o);
+        acc.x += __shfl_xor_sync(MB_FULL, acc.x, o);
+        acc.y += __shfl_xor_sync(MB_FULL, acc.y, o);
+        acc.z += __shfl_xor_sync(MB_FULL, acc.z, o);
+        acc.w += __shfl_xor_sync(MB_FULL, acc.w, o);
+    }
+    if (lane < columns) s_acc[warp][lane] = acc;
+    if (lane == 0) s_stat[warp] = make_float2(m, sum);
+    __syncthreads();
+    if (warp != 0 || lane >= columns || !mine) return;
+    const int warps = blockDim.x >> 5;
+    for (int o = 1; o < warps; ++o) m = fmaxf(m, s_stat[o].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    sum = 0.0f;
+    acc = make_float4(0, 0, 0, 0);
+    for (int o = 0; o < warps; ++o) {
+        const float g = pow2(s_stat[o].x - ref);
+        const float4 a = s_acc[o][lane];
+        sum = fmaf(s_stat[o].y, g, sum);
+        acc.x = fmaf(a.x, g, acc.x); acc.y = fmaf(a.y, g, acc.y);
+        acc.z = fmaf(a.z, g, acc.z); acc.w = fmaf(a.w, g, acc.w);
+    }
+    float *out = p.out + (size_t)b * p.out_stride + head * p.head_width + d;
+    out[0] = __fdiv_rn(acc.x, sum);
+    out[1] = __fdiv_rn(acc.y, sum);
+    out[2] = __fdiv_rn(acc.z, sum);
+    out[3] = __fdiv_rn(acc.w, sum);
 }
 
 struct Shape { int heads_per_cta, groups, phases, workers, lpr; };
@@ -373,10 +487,11 @@ template <typename T>
 int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
     const dim3 grid((unsigned)s.workers, (unsigned)s.groups), block((unsigned)(s.heads_per_cta * s.phases * 32));
     const size_t smem = ((size_t)p.lanes + 1u) * sizeof(unsigned);
-    if (s.lpr == 8) return mb_launch(k_lane_rows<T, 8>, grid, block, smem, stream, p);
-    if (s.lpr == 4) return mb_launch(k_lane_rows<T, 4>, grid, block, smem, stream, p);
-    if (s.lpr == 2) return mb_launch(k_lane_rows<T, 2>, grid, block, smem, stream, p);
-    return mb_launch(k_lane_rows<T, 1>, grid, block, smem, stream, p);
+    constexpr int U = sizeof(T) == 2 ? 2 : 1;
+    if (s.lpr == 8) return mb_launch(k_lane_rows<T, 8, U>, grid, block, smem, stream, p);
+    if (s.lpr == 4) return mb_launch(k_lane_rows<T, 4, U>, grid, block, smem, stream, p);
+    if (s.lpr == 2) return mb_launch(k_lane_rows<T, 2, U>, grid, block, smem, stream, p);
+    return mb_launch(k_lane_rows<T, 1, U>, grid, block, smem, stream, p);
 }
 
 size_t up4(size_t n) { return (n + 3u) & ~(size_t)3u; }
@@ -388,7 +503,7 @@ extern "C" size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t he
     (void)prefixes;
     (void)prefix_capacity;
     const Shape s = lane_shape(heads, head_width, sm_count);
-    const size_t parts = ((size_t)s.workers + lanes) * (size_t)s.phases;
+    const size_t parts = (size_t)s.workers + lanes;
     return up4(lanes + 2u) + up4(2u * parts * heads) + parts * heads * head_width;
 }
 
@@ -396,7 +511,7 @@ extern "C" int mb_lane_attention_init(void) { return 0; }
 
 extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     const Shape s = lane_shape(a->heads, a->head_width, a->sm_count);
-    const size_t parts = ((size_t)s.workers + a->lanes) * (size_t)s.phases;
+    const size_t parts = (size_t)s.workers + a->lanes;
     LaneP p = {};
     p.lanes = (int)a->lanes;
     p.heads = (int)a->heads;
@@ -435,10 +550,12 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     const cudaStream_t st = (cudaStream_t)stream;
     int rc = a->cache.type == MB_F16 ? launch_rows<__half>(p, s, st) : launch_rows<float>(p, s, st);
     if (rc != 0) return rc;
-    const unsigned warps = a->heads < 12u ? (unsigned)a->heads : 12u;
-    const dim3 grid((unsigned)a->lanes, 1u), block(warps * 32u);
-    rc = a->cache.type == MB_F16 ? mb_launch(k_lane_merge<__half>, grid, block, 0, st, p)
-                                 : mb_launch(k_lane_merge<float>, grid, block, 0, st, p);
+    int columns = 1;
+    while (columns * 4 < p.head_width) columns *= 2;
+    const size_t ctas = a->lanes * a->heads;
+    const dim3 grid((unsigned)a->lanes, (unsigned)a->heads), block(ctas <= 2u * (size_t)a->sm_count ? 512u : 128u);
+    rc = a->cache.type == MB_F16 ? mb_launch(k_lane_merge<__half>, grid, block, 0, st, p, columns)
+                                 : mb_launch(k_lane_merge<float>, grid, block, 0, st, p, columns);
     if (rc == 0 && a->launched != nullptr) *a->launched += 2u;
     return rc;
 }

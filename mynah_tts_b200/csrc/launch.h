@@ -384,7 +384,10 @@ typedef struct {
     const unsigned *live;       /* requests in use, or NULL */
     float *score_out;
     unsigned *token, *parent, *done_out;   /* done_out may be NULL */
+    const int *clusters;        /* host: mb_beam_init's */
 } mb_beam_select_args;
+/* clusters[1 .. 8]: how many clusters of that many CTAs the current device holds at once. */
+int mb_beam_init(int *clusters);
 int mb_beam_select(const mb_beam_select_args *args, mb_stream stream);
 
 typedef struct {
