@@ -63,8 +63,10 @@ static int attention_sizes_ok(size_t lanes, size_t heads, size_t head_width) {
 size_t mynah_b200_lane_attention_workspace(const void *state, size_t lanes, size_t heads, size_t head_width,
                                            size_t prefixes, size_t prefix_capacity) {
     const mb_state *st = (const mb_state *)state;
-    if (st == NULL || !attention_sizes_ok(lanes, heads, head_width) || prefix_capacity > 0xffffffffu / lanes) return 0;
-    return mb_lane_attention_floats(lanes, heads, head_width, prefixes, prefix_capacity, st->sm_count);
+    if (st == NULL || !attention_sizes_ok(lanes, heads, head_width) || prefixes > MB_LANES_MAX ||
+        prefix_capacity > 0xffffffffu / lanes)
+        return 0;
+    return mb_lane_attention_floats(lanes, heads, head_width, prefixes, st->sm_count);
 }
 
 int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args *a, char *error, size_t cap) {
@@ -96,8 +98,7 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
     if (a->window > 0 && (a->window > a->cache.capacity || a->sinks > a->cache.capacity - a->window))
         return refuse("a windowed cache must hold window + sinks rows", error, cap);
     if (a->dev_workspace == NULL || !aligned16(a->dev_workspace) ||
-        a->workspace_floats < mb_lane_attention_floats(a->lanes, a->heads, a->head_width, a->prefixes, prefix_capacity,
-                                                       st->sm_count))
+        a->workspace_floats < mb_lane_attention_floats(a->lanes, a->heads, a->head_width, a->prefixes, st->sm_count))
         return refuse("lane attention workspace is too small or not 16-byte aligned", error, cap);
     unsigned launched = 0;
     mb_lane_attn_args m;

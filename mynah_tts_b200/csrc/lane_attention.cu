@@ -45,6 +45,13 @@ struct LaneP {
     float2 *stat;                  // [part][heads] maximum, sum
     float *acc;                    // [part][heads][head_width]
     int heads_per_cta, phases;     // warps of a CTA: heads x row phases
+    // the prefixes on the tensor cores (lane_prefix.cuh); 0 workers: prefix rows are walked like own rows
+    int tile_workers;
+    unsigned *tile_lane;           // [lanes] rank among the lanes of its prefix
+    uint4 *tile_prefix;            // [prefixes]
+    unsigned *tile_run;
+    float2 *tile_stat;             // [partial row]
+    float *tile_acc;               // [partial row][head_width]
 };
 
 // What a lane sees of its cached rows.  Prefix row i of `prefix_rows` is row i below
@@ -130,6 +137,13 @@ __device__ __forceinline__ float pow2(float x) {
     return y;
 }
 
+// What is left of it for k_lane_rows.
+__device__ __forceinline__ LaneView lane_rows_view(const LaneP &p, int b) {
+    LaneView w = lane_view(p, b);
+    if (p.tile_workers > 0) w.prefix_rows = 0;
+    return w;
+}
+
 // Rows of the lanes, counted on, and the length of a run: every CTA forms them (lanes <= 1024).
 __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int workers, int step) {
     __shared__ unsigned warp_sum_s[32];
@@ -139,7 +153,7 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
         if (warp == 0) {
             unsigned n = 0;
             if (lane < p.lanes) {
-                const LaneView w = lane_view(p, lane);
+                const LaneView w = lane_rows_view(p, lane);
                 n = w.prefix_rows + w.own_rows;
             }
             unsigned x = n;
@@ -155,7 +169,7 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
         const int b = b0 + tid;
         unsigned n = 0;
         if (b < p.lanes) {
-            const LaneView w = lane_view(p, b);
+            const LaneView w = lane_rows_view(p, b);
             n = w.prefix_rows + w.own_rows;
         }
         unsigned x = n;
@@ -219,7 +233,7 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
     }
     const int group = lane / LPR, part = lane % LPR;
     while (at < end) {
-        const LaneView w = lane_view(p, b);
+        const LaneView w = lane_rows_view(p, b);
         const unsigned first = at - sm_off[b], last = min(end, sm_off[b + 1]) - sm_off[b];
         const T *pk = reinterpret_cast<const T *>(p.prefix_k) + w.prefix * p.prefix_stride + head * p.head_width;
         const T *pv = reinterpret_cast<const T *>(p.prefix_v) + w.prefix * p.prefix_stride + head * p.head_width;
@@ -355,18 +369,64 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
     }
 }
 
+}  // namespace
+
+#include "lane_prefix.cuh"
+
+namespace {
+
 // One CTA per head of a lane: the new row's score, the lane's partials, the result, and the new
 // row into the cache.  Four columns per thread, threads of the same columns take every
 // SLICES-th partial, MERGE_U at a time (a lane alone has hundreds).  A lane whose cache is full
 // or whose slot does not exist is left out and sets the status word.
 constexpr int MERGE_U = 4;
 
+struct Merged { float top, sum; float4 acc; };
+
+__device__ __forceinline__ void scale4(float4 &a, float f) { a.x *= f; a.y *= f; a.z *= f; a.w *= f; }
+__device__ __forceinline__ void add4(float4 &a, const float4 &b, float f) {
+    a.x = fmaf(b.x, f, a.x); a.y = fmaf(b.y, f, a.y); a.z = fmaf(b.z, f, a.z); a.w = fmaf(b.w, f, a.w);
+}
+
+// Joins the slices of a CTA; the result is in the first `columns` threads.
+__device__ __forceinline__ Merged join_slices(Merged r, int columns, float4 (*s_acc)[32], float2 *s_stat) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    float m = r.top;
+    for (int o = columns; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(MB_FULL, m, o));
+    const float f = pow2(r.top - (m == -INFINITY ? 0.0f : m));
+    r.sum *= f;
+    scale4(r.acc, f);
+    for (int o = columns; o < 32; o <<= 1) {
+        r.sum += __shfl_xor_sync(MB_FULL, r.sum, o);
+        r.acc.x += __shfl_xor_sync(MB_FULL, r.acc.x, o);
+        r.acc.y += __shfl_xor_sync(MB_FULL, r.acc.y, o);
+        r.acc.z += __shfl_xor_sync(MB_FULL, r.acc.z, o);
+        r.acc.w += __shfl_xor_sync(MB_FULL, r.acc.w, o);
+    }
+    if (lane < columns) s_acc[warp][lane] = r.acc;
+    if (lane == 0) s_stat[warp] = make_float2(m, r.sum);
+    __syncthreads();
+    r.top = m;
+    if (warp != 0 || lane >= columns) return r;
+    for (int o = 1; o < warps; ++o) r.top = fmaxf(r.top, s_stat[o].x);
+    const float ref = r.top == -INFINITY ? 0.0f : r.top;
+    r.sum = 0.0f;
+    r.acc = make_float4(0, 0, 0, 0);
+    for (int o = 0; o < warps; ++o) {
+        const float g = pow2(s_stat[o].x - ref);
+        r.sum = fmaf(s_stat[o].y, g, r.sum);
+        add4(r.acc, s_acc[o][lane], g);
+    }
+    return r;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
     __shared__ float4 s_acc[16][32];
     __shared__ float2 s_stat[16];
-    const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // lane state and rows were written before k_lane_rows began
+    __shared__ int s_again;
+    const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+    // lane state and rows were written before the first kernel of the call began
     if (p.live != nullptr && (unsigned)b >= *p.live) return;
     const LaneView w = lane_view(p, b);
     const int column = tid % columns, slice = tid / columns, slices = blockDim.x / columns;
@@ -374,14 +434,16 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
     const bool mine = d < p.head_width;
     const float *row = p.qkv + (size_t)b * p.qkv_stride + head * p.head_width + d;
     T kt[4], vt[4];
-    float x = 0.0f;
+    float q[4], x = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         kt[i] = (T)(mine ? row[p.width + i] : 0.0f);
         vt[i] = (T)(mine ? row[2 * p.width + i] : 0.0f);
-        x = fmaf(mine ? row[i] * p.scale_log2 : 0.0f, (float)kt[i], x);
+        q[i] = mine ? row[i] * p.scale_log2 : 0.0f;
+        x = fmaf(q[i], (float)kt[i], x);
     }
     for (int o = columns >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(MB_FULL, x, o);
+    if (tid == 0) s_again = 0;
     mb_pdl_wait();
     mb_pdl_trigger();
     if (!w.ok) {
@@ -390,20 +452,30 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
     }
     const unsigned first = p.offset[b], last = p.offset[b + 1], run = p.offset[p.lanes + 1];
     const unsigned part0 = last > first ? first / run : 0u;
-    const int n = last > first ? (int)((last - 1) / run - part0) + 1 : 0;
+    const int n_rows = last > first ? (int)((last - 1) / run - part0) + 1 : 0;
     const size_t base = (size_t)(part0 + b) * p.heads + head;
+    int n = n_rows;
+    size_t tile_base = 0;
+    if (p.tile_workers > 0 && w.prefix_rows > 0) {
+        const uint4 of = p.tile_prefix[w.prefix];
+        const unsigned rank = p.tile_lane[b], tile = rank / TILE, each = *p.tile_run;
+        const unsigned u0 = of.x + (tile * (unsigned)p.heads + (unsigned)head) * of.w, v0 = u0 / each;
+        n += (int)((u0 + of.w - 1u) / each - v0) + 1;
+        tile_base = of.y + (size_t)tile * TILE * p.heads + (size_t)head * min((unsigned)TILE, of.z - tile * TILE) +
+                    (size_t)v0 * TILE + rank % TILE;
+    }
+    const size_t at_new = w.slot * p.slot_stride + (size_t)w.append * p.row_stride + head * p.head_width + d;
     if (slice == 0 && mine) {
-        const size_t o = w.slot * p.slot_stride + (size_t)w.append * p.row_stride + head * p.head_width + d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            reinterpret_cast<T *>(p.k)[o + i] = kt[i];
-            reinterpret_cast<T *>(p.v)[o + i] = vt[i];
+            reinterpret_cast<T *>(p.k)[at_new + i] = kt[i];
+            reinterpret_cast<T *>(p.v)[at_new + i] = vt[i];
         }
     }
     // the first slice begins with the new row, the others with nothing
-    float top = slice == 0 ? x : -INFINITY, sum = slice == 0 ? 1.0f : 0.0f;
-    float4 acc = slice == 0 ? make_float4((float)vt[0], (float)vt[1], (float)vt[2], (float)vt[3]) : make_float4(0, 0, 0, 0);
-    if (slice == 0 && x == -INFINITY) { sum = 0.0f; acc = make_float4(0, 0, 0, 0); }
+    const Merged none = {-INFINITY, 0.0f, make_float4(0, 0, 0, 0)};
+    const Merged own = {x, 1.0f, make_float4((float)vt[0], (float)vt[1], (float)vt[2], (float)vt[3])};
+    Merged r = slice == 0 && x != -INFINITY ? own : none;
     for (int i0 = slice; i0 < n; i0 += MERGE_U * slices) {
         float2 s[MERGE_U];
         float4 a[MERGE_U];
@@ -412,62 +484,80 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
             const int i = i0 + u * slices;
             s[u] = make_float2(-INFINITY, 0.0f);
             a[u] = make_float4(0, 0, 0, 0);
-            if (i < n) {
+            if (i < n_rows) {
                 const size_t at = base + (size_t)i * p.heads;
                 s[u] = p.stat[at];
                 if (mine) a[u] = *reinterpret_cast<const float4 *>(p.acc + at * p.head_width + d);
+            } else if (i < n) {
+                const size_t at = tile_base + (size_t)(i - n_rows) * TILE;
+                s[u] = p.tile_stat[at];
+                if (mine) a[u] = *reinterpret_cast<const float4 *>(p.tile_acc + at * p.head_width + d);
             }
         }
-        float m = top;
+        float m = r.top;
 #pragma unroll
         for (int u = 0; u < MERGE_U; ++u) m = fmaxf(m, s[u].x);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        const float keep = pow2(top - ref);
-        top = m;
-        sum *= keep;
-        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+        const float ref = m == -INFINITY ? 0.0f : m, keep = pow2(r.top - ref);
+        r.top = m;
+        r.sum *= keep;
+        scale4(r.acc, keep);
 #pragma unroll
         for (int u = 0; u < MERGE_U; ++u) {
             const float f = pow2(s[u].x - ref);
-            sum = fmaf(s[u].y, f, sum);
-            acc.x = fmaf(a[u].x, f, acc.x); acc.y = fmaf(a[u].y, f, acc.y);
-            acc.z = fmaf(a[u].z, f, acc.z); acc.w = fmaf(a[u].w, f, acc.w);
+            r.sum = fmaf(s[u].y, f, r.sum);
+            add4(r.acc, a[u], f);
         }
     }
-    // slices of the warp, then of the other warps
-    float m = top;
-    for (int o = columns; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(MB_FULL, m, o));
-    const float f = pow2(top - (m == -INFINITY ? 0.0f : m));
-    sum *= f;
-    acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-    for (int o = columns; o < 32; o <<= 1) {
-        sum += __shfl_xor_sync(MB_FULL, sum, o);
-        acc.x += __shfl_xor_sync(MB_FULL, acc.x, o);
-        acc.y += __shfl_xor_sync(MB_FULL, acc.y, o);
-        acc.z += __shfl_xor_sync(MB_FULL, acc.z, o);
-        acc.w += __shfl_xor_sync(MB_FULL, acc.w, o);
-    }
-    if (lane < columns) s_acc[warp][lane] = acc;
-    if (lane == 0) s_stat[warp] = make_float2(m, sum);
-    __syncthreads();
-    if (warp != 0 || lane >= columns || !mine) return;
-    const int warps = blockDim.x >> 5;
-    for (int o = 1; o < warps; ++o) m = fmaxf(m, s_stat[o].x);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    sum = 0.0f;
-    acc = make_float4(0, 0, 0, 0);
-    for (int o = 0; o < warps; ++o) {
-        const float g = pow2(s_stat[o].x - ref);
-        const float4 a = s_acc[o][lane];
-        sum = fmaf(s_stat[o].y, g, sum);
-        acc.x = fmaf(a.x, g, acc.x); acc.y = fmaf(a.y, g, acc.y);
-        acc.z = fmaf(a.z, g, acc.z); acc.w = fmaf(a.w, g, acc.w);
-    }
+    r = join_slices(r, columns, s_acc, s_stat);
     float *out = p.out + (size_t)b * p.out_stride + head * p.head_width + d;
-    out[0] = __fdiv_rn(acc.x, sum);
-    out[1] = __fdiv_rn(acc.y, sum);
-    out[2] = __fdiv_rn(acc.z, sum);
-    out[3] = __fdiv_rn(acc.w, sum);
+    auto store = [&]() {
+        const float y[4] = {__fdiv_rn(r.acc.x, r.sum), __fdiv_rn(r.acc.y, r.sum), __fdiv_rn(r.acc.z, r.sum), __fdiv_rn(r.acc.w, r.sum)};
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            out[i] = y[i];
+            finite = finite && fabsf(y[i]) < INFINITY;
+        }
+        return finite;
+    };
+    const bool stores = tid < columns && mine;
+    if (stores && !store() && p.tile_workers > 0) s_again = 1;
+    if (p.tile_workers == 0) return;
+    __syncthreads();
+    if (s_again == 0) return;
+    // Infinities or NaN among the rows: a value kept as planes turns inf into inf - inf, so this
+    // head is formed once more from the values themselves, row by row.
+    const size_t prefix = (size_t)w.prefix * p.prefix_stride + head * p.head_width + d;
+    const size_t slot = w.slot * p.slot_stride + head * p.head_width + d;
+    r = slice == 0 && x != -INFINITY ? own : none;
+    for (unsigned i0 = 0; i0 < w.prefix_rows + w.own_rows; i0 += slices) {
+        const unsigned i = i0 + slice;
+        const bool in = i < w.prefix_rows + w.own_rows;
+        float kx[4] = {0, 0, 0, 0}, vx[4] = {0, 0, 0, 0}, y = 0.0f;
+        if (in && mine) {
+            const bool shared = i < w.prefix_rows;
+            const size_t at = shared ? prefix + (size_t)(i < w.prefix_head ? i : i + w.prefix_jump) * p.prefix_row_stride
+                                     : slot + (size_t)own_row(p, w, i - w.prefix_rows) * p.row_stride;
+            const T *k = reinterpret_cast<const T *>(shared ? p.prefix_k : p.k) + at;
+            const T *v = reinterpret_cast<const T *>(shared ? p.prefix_v : p.v) + at;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                kx[j] = (float)k[j];
+                vx[j] = (float)v[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y = fmaf(q[j], kx[j], y);
+        for (int o = columns >> 1; o > 0; o >>= 1) y += __shfl_xor_sync(MB_FULL, y, o);
+        if (!in) y = -INFINITY;
+        const float m = fmaxf(r.top, y), ref = m == -INFINITY ? 0.0f : m, keep = pow2(r.top - ref), e = pow2(y - ref);
+        r.top = m;
+        r.sum = fmaf(r.sum, keep, e);
+        scale4(r.acc, keep);
+        if (in) add4(r.acc, make_float4(vx[0], vx[1], vx[2], vx[3]), e);
+    }
+    r = join_slices(r, columns, s_acc, s_stat);
+    if (stores) store();
 }
 
 struct Shape { int heads_per_cta, groups, phases, workers, lpr; };
@@ -483,6 +573,40 @@ Shape lane_shape(size_t heads, size_t head_width, int sm_count) {
     return s;
 }
 
+// From TILE_LANES lanes the prefixes go through the tensor cores.
+constexpr size_t TILE_LANES = 16;
+
+int tile_workers(size_t lanes, size_t prefixes, int sm_count) {
+    return prefixes > 0 && lanes >= TILE_LANES ? TILE_CTAS_PER_SM * sm_count : 0;
+}
+
+// Places of the workspace, in floats.
+struct Places { size_t offset, stat, acc, tile_lane, tile_prefix, tile_run, tile_stat, tile_acc, floats; };
+
+Places lane_places(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count) {
+    const Shape s = lane_shape(heads, head_width, sm_count);
+    const size_t parts = (size_t)s.workers + lanes;
+    const size_t workers = (size_t)tile_workers(lanes, prefixes, sm_count);
+    const size_t rows = workers > 0 ? lanes * heads + workers * TILE : 0u;
+    Places w;
+    size_t at = 0;
+    auto take = [&at](size_t floats) {
+        const size_t from = at;
+        at += (floats + 3u) & ~(size_t)3u;
+        return from;
+    };
+    w.offset = take(lanes + 2u);
+    w.stat = take(2u * parts * heads);
+    w.acc = take(parts * heads * head_width);
+    w.tile_lane = take(workers > 0 ? lanes : 0u);
+    w.tile_prefix = take(workers > 0 ? 4u * prefixes : 0u);
+    w.tile_run = take(workers > 0 ? 1u : 0u);
+    w.tile_stat = take(2u * rows);
+    w.tile_acc = take(rows * head_width);
+    w.floats = at;
+    return w;
+}
+
 template <typename T>
 int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
     const dim3 grid((unsigned)s.workers, (unsigned)s.groups), block((unsigned)(s.heads_per_cta * s.phases * 32));
@@ -494,24 +618,54 @@ int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
     return mb_launch(k_lane_rows<T, 1, U>, grid, block, smem, stream, p);
 }
 
-size_t up4(size_t n) { return (n + 3u) & ~(size_t)3u; }
+template <typename T, int SLABS>
+size_t tile_smem(size_t lanes, size_t prefixes) {
+    return TileShape<T, SLABS>::SMEM + 16u * prefixes + 6u * lanes + 16u;
+}
+template <typename T, int SLABS>
+int launch_tiles(const LaneP &p, cudaStream_t stream) {
+    return mb_launch(k_lane_prefix<T, SLABS>, dim3((unsigned)p.tile_workers), dim3(TILE), tile_smem<T, SLABS>((size_t)p.lanes, p.prefixes),
+                     stream, p);
+}
+
+template <typename T>
+int launch_all(const LaneP &p, const Shape &s, int sm_count, cudaStream_t stream, unsigned *launched) {
+    int rc = 0;
+    if (p.tile_workers > 0) {
+        rc = p.head_width <= 64 ? launch_tiles<T, 1>(p, stream) : launch_tiles<T, 2>(p, stream);
+        if (rc != 0) return rc;
+    }
+    rc = launch_rows<T>(p, s, stream);
+    if (rc != 0) return rc;
+    int columns = 1;
+    while (columns * 4 < p.head_width) columns *= 2;
+    const size_t ctas = (size_t)p.lanes * (size_t)p.heads;
+    const dim3 grid((unsigned)p.lanes, (unsigned)p.heads), block(ctas <= 2u * (size_t)sm_count ? 512u : 128u);
+    rc = mb_launch(k_lane_merge<T>, grid, block, 0, stream, p, columns);
+    if (rc == 0 && launched != nullptr) *launched += p.tile_workers > 0 ? 3u : 2u;
+    return rc;
+}
 
 }  // namespace
 
-extern "C" size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes,
-                                           size_t prefix_capacity, int sm_count) {
-    (void)prefixes;
-    (void)prefix_capacity;
-    const Shape s = lane_shape(heads, head_width, sm_count);
-    const size_t parts = (size_t)s.workers + lanes;
-    return up4(lanes + 2u) + up4(2u * parts * heads) + parts * heads * head_width;
+extern "C" size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count) {
+    return lane_places(lanes, heads, head_width, prefixes, sm_count).floats;
 }
 
-extern "C" int mb_lane_attention_init(void) { return 0; }
+extern "C" int mb_lane_attention_init(void) {
+    const auto allow = [](auto kernel, size_t smem) {
+        return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    };
+    int rc = allow(k_lane_prefix<float, 1>, tile_smem<float, 1>(MB_LANES_MAX, MB_LANES_MAX));
+    if (rc == 0) rc = allow(k_lane_prefix<float, 2>, tile_smem<float, 2>(MB_LANES_MAX, MB_LANES_MAX));
+    if (rc == 0) rc = allow(k_lane_prefix<__half, 1>, tile_smem<__half, 1>(MB_LANES_MAX, MB_LANES_MAX));
+    if (rc == 0) rc = allow(k_lane_prefix<__half, 2>, tile_smem<__half, 2>(MB_LANES_MAX, MB_LANES_MAX));
+    return rc;
+}
 
 extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     const Shape s = lane_shape(a->heads, a->head_width, a->sm_count);
-    const size_t parts = (size_t)s.workers + a->lanes;
+    const Places w = lane_places(a->lanes, a->heads, a->head_width, a->prefixes, a->sm_count);
     LaneP p = {};
     p.lanes = (int)a->lanes;
     p.heads = (int)a->heads;
@@ -542,20 +696,18 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     p.out = a->out;
     p.out_stride = a->out_stride;
     p.status = a->status;
-    p.offset = reinterpret_cast<unsigned *>(a->workspace);
-    p.stat = reinterpret_cast<float2 *>(a->workspace + up4(a->lanes + 2u));
-    p.acc = a->workspace + up4(a->lanes + 2u) + up4(2u * parts * a->heads);
+    p.offset = reinterpret_cast<unsigned *>(a->workspace + w.offset);
+    p.stat = reinterpret_cast<float2 *>(a->workspace + w.stat);
+    p.acc = a->workspace + w.acc;
     p.heads_per_cta = s.heads_per_cta;
     p.phases = s.phases;
+    p.tile_workers = tile_workers(a->lanes, a->prefixes, a->sm_count);
+    p.tile_lane = reinterpret_cast<unsigned *>(a->workspace + w.tile_lane);
+    p.tile_prefix = reinterpret_cast<uint4 *>(a->workspace + w.tile_prefix);
+    p.tile_run = reinterpret_cast<unsigned *>(a->workspace + w.tile_run);
+    p.tile_stat = reinterpret_cast<float2 *>(a->workspace + w.tile_stat);
+    p.tile_acc = a->workspace + w.tile_acc;
     const cudaStream_t st = (cudaStream_t)stream;
-    int rc = a->cache.type == MB_F16 ? launch_rows<__half>(p, s, st) : launch_rows<float>(p, s, st);
-    if (rc != 0) return rc;
-    int columns = 1;
-    while (columns * 4 < p.head_width) columns *= 2;
-    const size_t ctas = a->lanes * a->heads;
-    const dim3 grid((unsigned)a->lanes, (unsigned)a->heads), block(ctas <= 2u * (size_t)a->sm_count ? 512u : 128u);
-    rc = a->cache.type == MB_F16 ? mb_launch(k_lane_merge<__half>, grid, block, 0, st, p, columns)
-                                 : mb_launch(k_lane_merge<float>, grid, block, 0, st, p, columns);
-    if (rc == 0 && a->launched != nullptr) *a->launched += 2u;
-    return rc;
+    return a->cache.type == MB_F16 ? launch_all<__half>(p, s, a->sm_count, st, a->launched)
+                                   : launch_all<float>(p, s, a->sm_count, st, a->launched);
 }

@@ -1,0 +1,429 @@
+// Shared-prefix part of the lane attention on the tensor cores: included by lane_attention.cu.
+//
+// The lanes of one prefix are rows of a tile (128 at most): for a head and a block of KEYS
+// prefix rows
+//     S = Q K^T,   p = 2^(S - max),   O += p V
+// with both products by tcgen05.mma, S, p and O in tensor memory.  The prefix is read once per
+// 128 lanes, which is the point; without it every lane would stream it.  Operands are 16-bit,
+// results are to be 32-bit: an f16 cache is exact as it is, and a query (first scaled by a power
+// of two into [1, 2)) and a weight are two f16 planes, 22 bits; an f32 cache, query and weight
+// are three bf16 planes, 24 bits and the exponent range of f32, and six of the nine products
+// (the others are below 2^-24 of the result).
+//
+// The blocks of all (tile, head) pairs, counted on, are cut into equal runs, one per CTA; a run
+// that ends inside a pair leaves a partial result, which k_lane_merge joins.  A thread owns a
+// row of the tile: its maximum, sum and weighted sum stay in registers, so tensor memory is never
+// rescaled.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "tc_common.cuh"
+
+namespace {
+
+constexpr int TILE = 128;          // rows of a tile, threads of a CTA
+constexpr unsigned TILE_TMEM = 256, TILE_O = 128;   // columns; S and p below, O from there on
+constexpr int TILE_CTAS_PER_SM = 2;
+
+template <typename T, int SLABS>
+struct TileShape {
+    static constexpr bool F16 = sizeof(T) == 2;
+    static constexpr int KEYS = F16 && SLABS == 1 ? 128 : 64;  // prefix rows of a block
+    static constexpr int QP = F16 ? 2 : 3, KP = F16 ? 1 : 3;   // planes of q and p, of K and V
+    static constexpr int Q_SLAB = TILE * 128, K_SLAB = KEYS * 128;     // bytes of 64 columns
+    static constexpr int Q_PLANE = SLABS * Q_SLAB, K_PLANE = SLABS * K_SLAB;
+    static constexpr size_t SMEM = (size_t)QP * Q_PLANE + 2u * KP * K_PLANE + 1024u;
+};
+
+__device__ __forceinline__ void tmem_ld32u(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+// Completes the loads issued so far; the registers pass through it so that no use moves in front.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+          "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+          "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+          "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+        :: "memory");
+}
+__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+// A from tensor memory, B from shared memory.
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Rows of 128 bytes (64 columns), 128-byte swizzle, read with the columns as the M or N
+// dimension: 8-row groups 1024 bytes apart along K, 64-column slabs `slab` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(unsigned addr, unsigned slab) {
+    uint64_t d = smem_desc_sw128(addr) & ~((uint64_t)0x3fff << 16);
+    return d | (uint64_t)((slab >> 4) & 0x3fffu) << 16;
+}
+
+// Two values into the QP 16-bit planes that sum to them.
+template <bool F16, int N>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&plane)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (F16) {
+            const __half2 h = __floats2half2_rn(a, b);
+            const float2 f = __half22float2(h);
+            plane[i] = *reinterpret_cast<const uint32_t *>(&h);
+            a -= f.x;
+            b -= f.y;
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            const float2 f = __bfloat1622float2(h);
+            plane[i] = *reinterpret_cast<const uint32_t *>(&h);
+            a -= f.x;
+            b -= f.y;
+        }
+    }
+}
+
+// Byte of 16-byte piece c of row r in a slab of 128-byte rows with 128-byte swizzle.
+__device__ __forceinline__ unsigned swizzled(int r, int c) { return (unsigned)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// Ranks of the lanes within their prefixes (in lane order; ~0u: no row of it to see) and, per
+// prefix, its first unit, its first row of partials, its lanes and its blocks.  A unit is one
+// block of one (tile, head) pair.  Worker v leaves its partial rows of a pair v * TILE rows
+// behind where the pair's rows begin: pairs and workers only go up along the units, so no two
+// partials meet.
+template <int KEYS>
+__device__ void tile_schedule(const LaneP &p, unsigned short *voice, unsigned *rank, uint4 *prefix, unsigned *units, unsigned *run) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    for (int g = tid; g < (int)p.prefixes; g += blockDim.x) {
+        const unsigned rows = min(p.prefix_length[g], p.prefix_capacity);
+        prefix[g] = make_uint4(0u, 0u, 0u, (rows + KEYS - 1) / KEYS);
+    }
+    for (int b = tid; b < p.lanes; b += blockDim.x) {
+        const LaneView w = lane_view(p, b);
+        voice[b] = w.prefix_rows > 0 ? (unsigned short)w.prefix : (unsigned short)0xffffu;
+    }
+    __syncthreads();
+    if (tid < 32) {
+        for (int b0 = 0; b0 < p.lanes; b0 += 32) {
+            const int b = b0 + lane;
+            const unsigned g = b < p.lanes ? voice[b] : 0xffffu;
+            const unsigned peers = __match_any_sync(MB_FULL, g);
+            const unsigned before = g != 0xffffu ? prefix[g].z : 0u;
+            __syncwarp();
+            if (b < p.lanes) rank[b] = g != 0xffffu ? before + __popc(peers & ((1u << lane) - 1u)) : 0xffffffffu;
+            if (g != 0xffffu && __ffs(peers) - 1 == lane) prefix[g].z = before + __popc(peers);
+            __syncwarp();
+        }
+        unsigned unit = 0, row = 0;
+        for (int g0 = 0; g0 < (int)p.prefixes; g0 += 32) {
+            const int g = g0 + lane;
+            uint4 v = g < (int)p.prefixes ? prefix[g] : make_uint4(0u, 0u, 0u, 0u);
+            const unsigned n = (v.z + TILE - 1) / TILE * (unsigned)p.heads * v.w;
+            unsigned x = n, y = v.z;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned a = __shfl_up_sync(MB_FULL, x, o), c = __shfl_up_sync(MB_FULL, y, o);
+                if (lane >= o) { x += a; y += c; }
+            }
+            v.x = unit + x - n;
+            v.y = row + (y - v.z) * (unsigned)p.heads;
+            if (g < (int)p.prefixes) prefix[g] = v;
+            unit += __shfl_sync(MB_FULL, x, 31);
+            row += __shfl_sync(MB_FULL, y, 31) * (unsigned)p.heads;
+        }
+        if (lane == 0) {
+            *units = unit;
+            *run = max((unit + p.tile_workers - 1) / p.tile_workers, 1u);
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, int SLABS>
+__global__ void __launch_bounds__(TILE, TILE_CTAS_PER_SM) k_lane_prefix(LaneP p) {
+    using C = TileShape<T, SLABS>;
+    constexpr bool F16 = C::F16;
+    constexpr int KEYS = C::KEYS, QP = C::QP, KP = C::KP;
+    extern __shared__ unsigned char sm_tile[];
+    __shared__ __align__(8) unsigned long long s_bar;
+    __shared__ uint32_t s_tmem;
+    __shared__ unsigned s_units, s_run;
+    __shared__ unsigned short s_row[TILE];                 // lanes of the tile
+    unsigned char *base = sm_tile + ((1024u - (saddr(sm_tile) & 1023u)) & 1023u);
+    unsigned char *sq = base, *sk = sq + QP * C::Q_PLANE, *sv = sk + KP * C::K_PLANE;
+    unsigned char *rest = base + (C::SMEM - 1024u);        // schedule
+    uint4 *s_prefix = reinterpret_cast<uint4 *>(rest);
+    unsigned *s_rank = reinterpret_cast<unsigned *>(s_prefix + p.prefixes);
+    unsigned short *s_voice = reinterpret_cast<unsigned short *>(s_rank + p.lanes);
+    const int tid = threadIdx.x, warp = tid >> 5;
+    mb_pdl_wait();
+    mb_pdl_trigger();
+    tile_schedule<KEYS>(p, s_voice, s_rank, s_prefix, &s_units, &s_run);
+    if (blockIdx.x == 0) {
+        for (int b = tid; b < p.lanes; b += TILE) p.tile_lane[b] = s_rank[b];
+        for (int g = tid; g < (int)p.prefixes; g += TILE) p.tile_prefix[g] = s_prefix[g];
+        if (tid == 0) *p.tile_run = s_run;
+    }
+    const unsigned units = s_units, run = s_run;
+    if ((unsigned long long)blockIdx.x * run >= units) return;
+    unsigned unit = blockIdx.x * run;
+    const unsigned end = min(units, unit + run);
+    if (tid == 0) {
+        bar_init(&s_bar, 1u);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&s_tmem)), "r"(TILE_TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem, my_tmem = tmem + ((uint32_t)(warp * 32) << 16);
+    const int hw = p.head_width, ksteps = (hw + 15) / 16, ncols = ksteps * 16;
+    const uint32_t format = F16 ? 0u : (1u << 7 | 1u << 10);
+    const uint32_t idesc_s = instr_desc_f16(TILE, KEYS) | format;
+    const uint32_t idesc_o = instr_desc_f16(TILE, ncols) | format | 1u << 16;          // B along N
+    unsigned parity = 0;
+    bool fine = true;
+    int g = 0;
+
+    while (unit < end && fine) {
+        while (g + 1 < (int)p.prefixes && s_prefix[g + 1].x <= unit) ++g;
+        const uint4 of = s_prefix[g];
+        const unsigned pair = (unit - of.x) / of.w, tile = pair / (unsigned)p.heads;
+        const int head = (int)(pair - tile * (unsigned)p.heads);
+        unsigned block = unit - of.x - pair * of.w;
+        const unsigned stop = min(of.w, block + (end - unit));
+        const int rows = (int)min((unsigned)TILE, of.z - tile * TILE);
+        const unsigned keys = min(p.prefix_length[g], p.prefix_capacity);
+        unit += stop - block;
+        __syncthreads();                                   // s_row, and the operands of the last block
+        for (int b = tid; b < p.lanes; b += TILE)
+            if (s_voice[b] == g && s_rank[b] / TILE == tile) s_row[s_rank[b] % TILE] = (unsigned short)b;
+        __syncthreads();
+
+        // this thread's query: scaled, cut into planes, rows of 128 bytes per slab
+        const bool mine = tid < rows;
+        unsigned seen_head = 0, seen_from = 0;             // rows of the prefix it sees: below, and from there on
+        float unscale = 1.0f;
+        {
+            const int b = mine ? s_row[tid] : 0;
+            const float *q = p.qkv + (size_t)b * p.qkv_stride + head * hw;
+            float up = 1.0f;
+            if (mine) {
+                const LaneView w = lane_view(p, b);
+                seen_head = w.prefix_head;
+                seen_from = w.prefix_head + w.prefix_jump;
+                if (F16) {
+                    float most = 0.0f;
+                    for (int d = 0; d < hw; ++d) most = fmaxf(most, fabsf(q[d] * p.scale_log2));
+                    // 2^e <= most < 2^(e + 1); zero and what is not finite stay as they are
+                    const int e = (int)(__float_as_uint(most) >> 23) - 127;
+                    if (e > -126 && e < 127) {
+                        up = __uint_as_float((unsigned)(127 - e) << 23);
+                        unscale = __uint_as_float((unsigned)(127 + e) << 23);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < SLABS * 8; ++c) {
+                uint32_t plane[4][QP];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = c * 8 + 2 * i;
+                    const float x = mine && d < hw ? q[d] * p.scale_log2 * up : 0.0f;
+                    const float y = mine && d + 1 < hw ? q[d + 1] * p.scale_log2 * up : 0.0f;
+                    split_pair<F16>(x, y, plane[i]);
+                }
+#pragma unroll
+                for (int j = 0; j < QP; ++j)
+                    *reinterpret_cast<uint4 *>(sq + j * C::Q_PLANE + (c >> 3) * C::Q_SLAB + swizzled(tid, c & 7)) =
+                        make_uint4(plane[0][j], plane[1][j], plane[2][j], plane[3][j]);
+            }
+        }
+        float top = -INFINITY, sum = 0.0f, o[SLABS * 64];
+#pragma unroll
+        for (int i = 0; i < SLABS * 64; ++i) o[i] = 0.0f;
+
+        for (; block < stop; ++block) {
+            const unsigned first = block * KEYS;
+            // K and V rows, zero beyond the prefix and beyond the head (unseen rows may hold anything)
+            const size_t origin = (size_t)g * p.prefix_stride + (size_t)head * hw;
+            const T *pk = reinterpret_cast<const T *>(p.prefix_k) + origin, *pv = reinterpret_cast<const T *>(p.prefix_v) + origin;
+#pragma unroll 4
+            for (int i = tid; i < KEYS * SLABS * 8; i += TILE) {
+                const int r = i / (SLABS * 8), c = i % (SLABS * 8), d = c * 8;
+                const bool in = first + r < keys;
+                const size_t at = (size_t)(first + r) * p.prefix_row_stride + d;
+                const unsigned to = (c >> 3) * C::K_SLAB + swizzled(r, c & 7);
+                if (F16) {
+                    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+                    if (in && d < hw) {
+                        x = __ldg(reinterpret_cast<const uint4 *>(pk + at));
+                        y = __ldg(reinterpret_cast<const uint4 *>(pv + at));
+                    }
+                    *reinterpret_cast<uint4 *>(sk + to) = x;
+                    *reinterpret_cast<uint4 *>(sv + to) = y;
+                } else {
+                    float4 x[4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        x[j] = x[2 + j] = make_float4(0, 0, 0, 0);
+                        if (in && d + 4 * j < hw) {
+                            x[j] = __ldg(reinterpret_cast<const float4 *>(pk + at + 4 * j));
+                            x[2 + j] = __ldg(reinterpret_cast<const float4 *>(pv + at + 4 * j));
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        uint32_t plane[4][KP];
+                        split_pair<F16>(x[2 * m].x, x[2 * m].y, plane[0]);
+                        split_pair<F16>(x[2 * m].z, x[2 * m].w, plane[1]);
+                        split_pair<F16>(x[2 * m + 1].x, x[2 * m + 1].y, plane[2]);
+                        split_pair<F16>(x[2 * m + 1].z, x[2 * m + 1].w, plane[3]);
+#pragma unroll
+                        for (int j = 0; j < KP; ++j)
+                            *reinterpret_cast<uint4 *>((m ? sv : sk) + j * C::K_PLANE + to) =
+                                make_uint4(plane[0][j], plane[1][j], plane[2][j], plane[3][j]);
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncthreads();
+            if (tid == 0) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t more = 0u;
+#pragma unroll
+                for (int a = 0; a < QP; ++a)
+#pragma unroll
+                    for (int b = 0; b < KP; ++b) {
+                        if (!F16 && a + b > 2) continue;
+                        for (int s = 0; s < ksteps; ++s) {
+                            const unsigned slab = s >> 2, off = (s & 3) * 32u;
+                            mma_f16(tmem, smem_desc_sw128(saddr(sq) + a * C::Q_PLANE + slab * C::Q_SLAB + off),
+                                    smem_desc_sw128(saddr(sk) + b * C::K_PLANE + slab * C::K_SLAB + off), idesc_s, more);
+                            more = 1u;
+                        }
+                    }
+                mma_commit(&s_bar);
+            }
+            bool done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
+            parity ^= 1u;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float keep = 1.0f;
+            if (done && warp * 32 < rows) {                // a warp without a row has nothing to weigh
+                uint32_t x[KEYS / 32][32];
+#pragma unroll
+                for (int i = 0; i < KEYS / 32; ++i) tmem_ld32u(my_tmem + i * 32, x[i]);
+#pragma unroll
+                for (int i = 0; i < KEYS / 32; ++i) tmem_ld_wait(x[i]);
+                // masked: beyond the prefix, or between the first rows and the window
+                const bool all = first + KEYS <= keys && (first + KEYS <= seen_head || first >= seen_from);
+                float m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) {
+                    const unsigned j = first + i;
+                    if (!all && !(j < keys && (j < seen_head || j >= seen_from))) x[i / 32][i % 32] = 0xff800000u;
+                    m = fmaxf(m, __uint_as_float(x[i / 32][i % 32]));
+                }
+                m = fmaxf(top, m * unscale);
+                const float ref = m == -INFINITY ? 0.0f : m;
+                keep = pow2(top - ref);
+                top = m;
+                sum *= keep;
+#pragma unroll
+                for (int i = 0; i < KEYS / 64; ++i) {
+                    uint32_t out[QP][32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int k = i * 64 + 2 * j;
+                        const float a = pow2(fmaf(__uint_as_float(x[k / 32][k % 32]), unscale, -ref));
+                        const float b = pow2(fmaf(__uint_as_float(x[(k + 1) / 32][(k + 1) % 32]), unscale, -ref));
+                        sum += a + b;
+                        uint32_t plane[QP];
+                        split_pair<F16>(a, b, plane);
+#pragma unroll
+                        for (int l = 0; l < QP; ++l) out[l][j] = plane[l];
+                    }
+#pragma unroll
+                    for (int l = 0; l < QP; ++l) tmem_st32u(my_tmem + l * (KEYS / 2) + i * 32, out[l]);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            fine = __syncthreads_and(done);
+            if (!fine) break;
+            if (tid == 0) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t more = 0u;
+#pragma unroll
+                for (int a = 0; a < QP; ++a)
+#pragma unroll
+                    for (int b = 0; b < KP; ++b) {
+                        if (!F16 && a + b > 2) continue;
+#pragma unroll
+                        for (int s = 0; s < KEYS / 16; ++s) {
+                            mma_f16_ts(tmem + TILE_O, tmem + a * (KEYS / 2) + s * 8,
+                                       smem_desc_sw128_mn(saddr(sv) + b * C::K_PLANE + s * 2048u, C::K_SLAB), idesc_o, more);
+                            more = 1u;
+                        }
+                    }
+                mma_commit(&s_bar);
+            }
+            done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
+            parity ^= 1u;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (done && warp * 32 < rows) {
+#pragma unroll
+                for (int i = 0; i < SLABS * 2; ++i) {
+                    if (i * 32 >= ncols) break;
+                    uint32_t x[32];
+                    tmem_ld32u(my_tmem + TILE_O + i * 32, x);
+                    tmem_ld_wait(x);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[i * 32 + j] = fmaf(o[i * 32 + j], keep, __uint_as_float(x[j]));
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            fine = __syncthreads_and(done);
+            if (!fine) break;
+        }
+        if (mine && fine) {
+            const size_t at = of.y + (size_t)tile * TILE * p.heads + (size_t)head * rows + (size_t)blockIdx.x * TILE + tid;
+            p.tile_stat[at] = make_float2(top, sum);
+#pragma unroll
+            for (int i = 0; i < SLABS * 64; i += 4)
+                if (i < hw) *reinterpret_cast<float4 *>(p.tile_acc + at * hw + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+    }
+    if (!fine && tid == 0) {
+        atomicOr(p.status, 16);
+        bar_wait(&s_bar, parity ^ 1u, TC_SPIN >> 4);       // what may still be in flight, one more bounded chance
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 0)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TILE_TMEM) : "memory");
+}
+
+}  // namespace

@@ -424,8 +424,7 @@ typedef struct {
     int sm_count;
     unsigned *launched;         /* incremented by the number of kernels the call enqueued */
 } mb_lane_attn_args;
-size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes, size_t prefix_capacity,
-                                int sm_count);
+size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count);
 int mb_lane_attention_init(void);
 int mb_lane_attention(const mb_lane_attn_args *args, mb_stream stream);
 
