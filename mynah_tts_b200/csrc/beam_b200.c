@@ -36,7 +36,7 @@ static int check_cache(const mynah_b200_lane_cache *c, int layers, char *error, 
     const size_t per = c->type == MYNAH_B200_F16 ? 8u : 4u;
     if (c->dev_k == NULL || c->dev_v == NULL || c->slots == 0 || c->capacity == 0 || c->width == 0)
         return refuse("lane cache is empty", error, cap);
-    if (c->slots > 0xffffffffu || c->capacity > 0x7fffffffu || c->width > 0x7fffffffu)
+    if (c->slots > 0xffffffffu || c->capacity > 0x7fffffffu || c->row_stride > 0x1fffffffu)
         return refuse("lane cache is too large", error, cap);
     if (c->row_stride < c->width || c->width % per != 0 || c->row_stride % per != 0 || c->slot_stride % per != 0 ||
         !aligned16(c->dev_k) || !aligned16(c->dev_v))
@@ -87,7 +87,7 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
     if (a->prefixes > 0) {
         prefix_capacity = a->prefix_capacity;
         if (a->prefixes > MB_LANES_MAX || a->dev_prefix_k == NULL || a->dev_prefix_v == NULL || a->dev_prefix_length == NULL ||
-            prefix_capacity == 0 || prefix_capacity > 0x7fffffffu)
+            prefix_capacity == 0 || prefix_capacity > 0x7fffffffu || a->prefix_row_stride > 0x1fffffffu)
             return refuse("invalid lane attention prefixes", error, cap);
         if (a->prefix_row_stride < width || a->prefix_row_stride % per != 0 || a->prefix_stride % per != 0 ||
             (a->prefixes > 1 && a->prefix_stride == 0) || !aligned16(a->dev_prefix_k) || !aligned16(a->dev_prefix_v))

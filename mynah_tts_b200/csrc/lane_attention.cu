@@ -16,6 +16,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "tc_common.cuh"
 
 namespace {
 
@@ -45,6 +46,7 @@ struct LaneP {
     float2 *stat;                  // [part][heads] maximum, sum
     float *acc;                    // [part][heads][head_width]
     int heads_per_cta, phases;     // warps of a CTA: heads x row phases
+    int step, row_bytes, row_pitch;      // rows of a step; bytes of a row's heads of a CTA, and between rows in the ring
     // the prefixes on the tensor cores (lane_prefix.cuh); 0 workers: prefix rows are walked like own rows
     int tile_workers;
     unsigned *tile_lane;           // [lanes] rank among the lanes of its prefix
@@ -198,29 +200,57 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
 }
 
 // LPR lanes of a warp share a row's head (16 elements each), so a warp takes 32 / LPR rows at
-// a time, U times over before it uses them; a row's score is complete in its lanes after
-// log2(LPR) exchanges, and every group of LPR lanes keeps its own running maximum and sum,
-// joined once per run.  Few heads: `phases` warps share a head's rows and join through shared
-// memory.
-template <typename T, int LPR, int U>
-__global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP p) {
-    extern __shared__ unsigned sm_off[];
+// a time, U times over; a row's score is complete in its lanes after log2(LPR) exchanges, and
+// every group of LPR lanes keeps its own running maximum and sum, joined once per run.  Few
+// heads: `phases` warps share a head's rows and join through shared memory.
+//
+// A warp of its own brings the rows, all heads of a CTA in one bulk copy, into a ring of
+// ROWS_DEPTH steps, across the lanes of a run: up to 100 KB per CTA, two CTAs per SM.  Rows lie
+// row_pitch apart there, an odd multiple of the 16 * LPR bytes that the lanes of a row read at
+// once (any 16-byte multiple for eight lanes), so that a warp's reads share no bank.
+// (48 lanes x 1,029 f16 rows, 152 MB, with the merge: loads into registers 40 us, 16-byte copies
+// by every thread 34 us, bulk copies ROWS_US us.)
+constexpr int ROWS_DEPTH = 2;
+constexpr size_t ROWS_STAGE = 50u * 1024u;       // bytes of a step, at most
+
+template <typename T>
+constexpr int ROWS_U = sizeof(T) == 2 ? 2 : 1;   // rows of a group of lanes in a step
+
+__device__ __forceinline__ void copy_row(unsigned to, const char *from, unsigned bytes, void *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from),
+                 "r"(bytes), "r"(saddr(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(void *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(bar)) : "memory");
+}
+
+// FULL: the head fills all columns, LPR * 16.
+template <typename T, int LPR, bool FULL>
+__global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows(LaneP p) {
+    extern __shared__ uint4 sm_rows_dyn[];
     __shared__ unsigned s_run;
     __shared__ float s_acc[WARPS_MAX][MB_LANE_HEAD_WIDTH_MAX];
     __shared__ float2 s_stat[WARPS_MAX];
-    constexpr int PER = Piece<T>::N, V = 16 / PER, GROUPS = 32 / LPR;
+    __shared__ __align__(8) unsigned long long s_full[ROWS_DEPTH], s_empty[ROWS_DEPTH];
+    constexpr int PER = Piece<T>::N, V = 16 / PER, U = ROWS_U<T>, GROUPS = 32 / LPR;
+    unsigned *sm_off = reinterpret_cast<unsigned *>(sm_rows_dyn);
+    const char *ring = reinterpret_cast<const char *>(sm_rows_dyn + (p.lanes + 1 + 3) / 4);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = p.heads_per_cta * p.phases, step = p.step;
+    const unsigned plane = (unsigned)(step * p.row_pitch);       // K rows of a stage, then V rows
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ROWS_DEPTH; ++i) {
+            bar_init(&s_full[i], 1u);
+            bar_init(&s_empty[i], (unsigned)warps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     mb_pdl_wait();
     mb_pdl_trigger();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int step = GROUPS * U * p.phases;
     lane_schedule(p, sm_off, &s_run, gridDim.x, GROUPS * p.phases);
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         for (int i = threadIdx.x; i <= p.lanes; i += blockDim.x) p.offset[i] = sm_off[i];
         if (threadIdx.x == 0) p.offset[p.lanes + 1] = s_run;
     }
-    // a warp without a head (the last CTA row's) works on the last one and stores nothing
-    const int wanted = blockIdx.y * p.heads_per_cta + warp % p.heads_per_cta, phase = warp / p.heads_per_cta;
-    const int head = min(wanted, p.heads - 1);
     const unsigned total = sm_off[p.lanes], run = s_run;
     const unsigned long long begin = (unsigned long long)blockIdx.x * run;
     if (begin >= total) return;
@@ -231,62 +261,86 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
         const int mid = (lo + hi + 1) >> 1;
         if (sm_off[mid] <= at) lo = b = mid; else hi = mid - 1;
     }
-    const int group = lane / LPR, part = lane % LPR;
+    int stage = 0;
+    unsigned parity = 0;
+
+    if (warp == warps) {                         // brings the rows
+        const size_t column = (size_t)blockIdx.y * p.heads_per_cta * p.head_width * sizeof(T);
+        // the last group of heads may be smaller
+        const unsigned bytes = (unsigned)min((size_t)p.row_bytes, (size_t)p.width * sizeof(T) - column);
+        const ptrdiff_t own_v = p.v - p.k, shared_v = p.prefix_v - p.prefix_k;      // from a row of K to its row of V
+        bool fine = true;
+        for (unsigned steps = 0; at < end && fine; ++b) {
+            if (sm_off[b + 1] <= at) continue;
+            unsigned r0 = at - sm_off[b];
+            const unsigned last = min(end, sm_off[b + 1]) - sm_off[b];
+            const LaneView w = lane_rows_view(p, b);
+            const char *own = p.k + w.slot * p.slot_stride * sizeof(T) + column;
+            const char *shared = p.prefix_k + w.prefix * p.prefix_stride * sizeof(T) + column;
+            at += last - r0;
+            for (; r0 < last && fine; r0 += step) {
+                if (steps++ >= ROWS_DEPTH) fine = __all_sync(MB_FULL, bar_wait(&s_empty[stage], parity ^ 1u, TC_SPIN));
+                if (!fine) break;
+                const unsigned n = min((unsigned)step, last - r0);
+                if (lane == 0) bar_expect(&s_full[stage], 2u * n * bytes);
+                __syncwarp();
+                const unsigned to = saddr(ring) + (unsigned)stage * 2u * plane;
+                for (unsigned i = lane; i < n; i += 32) {
+                    const unsigned r = r0 + i;
+                    const bool first = r < w.prefix_rows;
+                    const size_t row = first ? (r < w.prefix_head ? r : r + w.prefix_jump) : own_row(p, w, r - w.prefix_rows);
+                    const char *k = first ? shared + row * p.prefix_row_stride * sizeof(T) : own + row * p.row_stride * sizeof(T);
+                    copy_row(to + i * p.row_pitch, k, bytes, &s_full[stage]);
+                    copy_row(to + plane + i * p.row_pitch, k + (first ? shared_v : own_v), bytes, &s_full[stage]);
+                }
+                if (++stage == ROWS_DEPTH) { stage = 0; parity ^= 1u; }
+            }
+        }
+        if (!fine && lane == 0) atomicOr(p.status, 2);
+        return;
+    }
+
+    // a warp without a head (of the last group) works on the last one and stores nothing
+    const int wanted = blockIdx.y * p.heads_per_cta + warp % p.heads_per_cta, phase = warp / p.heads_per_cta;
+    const bool has_head = wanted < p.heads;
+    const int head = min(wanted, p.heads - 1), group = lane / LPR, part = lane % LPR;
+    const char *mine = ring + (size_t)((head - blockIdx.y * p.heads_per_cta) * p.head_width + part * PER) * sizeof(T);
     while (at < end) {
-        const LaneView w = lane_rows_view(p, b);
         const unsigned first = at - sm_off[b], last = min(end, sm_off[b + 1]) - sm_off[b];
-        const T *pk = reinterpret_cast<const T *>(p.prefix_k) + w.prefix * p.prefix_stride + head * p.head_width;
-        const T *pv = reinterpret_cast<const T *>(p.prefix_v) + w.prefix * p.prefix_stride + head * p.head_width;
-        const T *ok = reinterpret_cast<const T *>(p.k) + w.slot * p.slot_stride + head * p.head_width;
-        const T *ov = reinterpret_cast<const T *>(p.v) + w.slot * p.slot_stride + head * p.head_width;
+        if (last == first) { ++b; continue; }
         float q[16], acc[16], top = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int d = ((i / PER) * LPR + part) * PER + i % PER;
-            q[i] = d < p.head_width ? p.qkv[(size_t)b * p.qkv_stride + head * p.head_width + d] * p.scale_log2 : 0.0f;
+            q[i] = FULL || d < p.head_width ? p.qkv[(size_t)b * p.qkv_stride + head * p.head_width + d] * p.scale_log2 : 0.0f;
             acc[i] = 0.0f;
         }
-        for (unsigned r0 = first + phase * GROUPS; r0 < last; r0 += step) {
-            uint4 kx[U][V], vx[U][V];
-            bool in[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const unsigned r = r0 + u * GROUPS * p.phases + group;
-                in[u] = r < last;
-                const T *rk = ok, *rv = ov;
-                if (r < w.prefix_rows) {
-                    const size_t o = (size_t)(r < w.prefix_head ? r : r + w.prefix_jump) * p.prefix_row_stride;
-                    rk = pk + o;
-                    rv = pv + o;
-                } else {
-                    const size_t o = (size_t)own_row(p, w, r - w.prefix_rows) * p.row_stride;
-                    rk = ok + o;
-                    rv = ov + o;
-                }
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int d = (j * LPR + part) * PER;
-                    kx[u][j] = vx[u][j] = make_uint4(0, 0, 0, 0);
-                    if (in[u] && d < p.head_width) {
-                        kx[u][j] = __ldg(reinterpret_cast<const uint4 *>(rk + d));
-                        vx[u][j] = __ldg(reinterpret_cast<const uint4 *>(rv + d));
-                    }
-                }
+        for (unsigned r0 = first; r0 < last; r0 += step) {
+            const bool there = __all_sync(MB_FULL, bar_wait(&s_full[stage], parity, TC_SPIN));
+            if (!there) {                        // what is still on its way gets no second chance to be waited for: TC_SPIN is seconds
+                if (lane == 0) atomicOr(p.status, 2);
+                return;
             }
+            const char *from = mine + (size_t)stage * 2u * plane;
+            const unsigned most = min((unsigned)step, last - r0) - 1u;
             float x[U], m = top;
+            const char *at_u[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                const unsigned i = (phase + u * p.phases) * GROUPS + group;
+                at_u[u] = from + (size_t)(min(i, most) * p.row_pitch);         // no row: the last one, with weight 0
                 x[u] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
+                    if (!FULL && (j * LPR + part) * PER >= p.head_width) continue;
                     float k[PER];
-                    Piece<T>::get(kx[u][j], k);
+                    Piece<T>::get(*reinterpret_cast<const uint4 *>(at_u[u] + j * LPR * 16), k);
 #pragma unroll
-                    for (int i = 0; i < PER; ++i) x[u] = fmaf(q[j * PER + i], k[i], x[u]);
+                    for (int e = 0; e < PER; ++e) x[u] = fmaf(q[j * PER + e], k[e], x[u]);
                 }
 #pragma unroll
                 for (int o = LPR / 2; o > 0; o >>= 1) x[u] += __shfl_xor_sync(MB_FULL, x[u], o);
-                if (!in[u]) x[u] = -INFINITY;
+                if (i > most) x[u] = -INFINITY;
                 m = fmaxf(m, x[u]);
             }
             const float ref = m == -INFINITY ? 0.0f : m;      // nothing but -inf so far: weights 0, not NaN
@@ -301,12 +355,16 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
                 sum += e;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
+                    if (!FULL && (j * LPR + part) * PER >= p.head_width) continue;
                     float v[PER];
-                    Piece<T>::get(vx[u][j], v);
+                    Piece<T>::get(*reinterpret_cast<const uint4 *>(at_u[u] + plane + j * LPR * 16), v);
 #pragma unroll
                     for (int i = 0; i < PER; ++i) acc[j * PER + i] = fmaf(e, v[i], acc[j * PER + i]);
                 }
             }
+            __syncwarp();
+            if (lane == 0) bar_arrive(&s_empty[stage]);
+            if (++stage == ROWS_DEPTH) { stage = 0; parity ^= 1u; }
         }
         // join the groups of the warp, then its phases
         float m = top;
@@ -329,7 +387,7 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s_acc[warp][((i / PER) * LPR + part) * PER + i % PER] = acc[i];
             }
-            __syncthreads();
+            asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
             if (phase == 0) {
                 float all = m;
                 for (int o = 1; o < p.phases; ++o) all = fmaxf(all, s_stat[warp + o * p.heads_per_cta].x);
@@ -348,15 +406,15 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
                 }
                 m = all;
             }
-            __syncthreads();
+            asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
         }
-        if (group == 0 && phase == 0 && wanted < p.heads) {
+        if (group == 0 && phase == 0 && has_head) {
             const size_t slot = (size_t)(blockIdx.x + b) * p.heads + head;
             if (part == 0) p.stat[slot] = make_float2(m, sum);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const int d = (j * LPR + part) * PER;
-                if (d < p.head_width)
+                if (FULL || d < p.head_width)
 #pragma unroll
                     for (int i = 0; i < PER; i += 4)
                         *reinterpret_cast<float4 *>(p.acc + slot * p.head_width + d + i) =
@@ -364,8 +422,7 @@ __global__ void __launch_bounds__(WARPS_MAX * 32, CTAS_PER_SM) k_lane_rows(LaneP
             }
         }
         at += last - first;
-        if (at < end)
-            do ++b; while (sm_off[b + 1] <= at);
+        ++b;
     }
 }
 
@@ -560,16 +617,22 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
     if (stores) store();
 }
 
-struct Shape { int heads_per_cta, groups, phases, workers, lpr; };
+struct Shape { int heads_per_cta, groups, phases, workers, lpr, step, row_bytes, row_pitch; };
 
-Shape lane_shape(size_t heads, size_t head_width, int sm_count) {
+Shape lane_shape(size_t heads, size_t head_width, size_t size, int sm_count) {
     Shape s;
     s.groups = (int)((heads + WARPS_MAX - 1) / WARPS_MAX);
     s.heads_per_cta = (int)((heads + s.groups - 1) / s.groups);
-    s.phases = WARPS_MAX / s.heads_per_cta;
     s.workers = CTAS_PER_SM * sm_count / s.groups;
     if (s.workers < 1) s.workers = 1;
     s.lpr = head_width > 64 ? 8 : head_width > 32 ? 4 : head_width > 16 ? 2 : 1;
+    s.row_bytes = (int)(s.heads_per_cta * head_width * size);
+    const int once = 16 * s.lpr, times = (s.row_bytes + once - 1) / once;
+    s.row_pitch = s.lpr < 8 ? (times | 1) * once : s.row_bytes;
+    const int rows = 32 / s.lpr * (size == 2 ? ROWS_U<__half> : ROWS_U<float>);        // of a warp in a step
+    s.phases = WARPS_MAX / s.heads_per_cta;
+    while (s.phases > 1 && 2u * (size_t)s.row_pitch * rows * s.phases > ROWS_STAGE) --s.phases;
+    s.step = rows * s.phases;
     return s;
 }
 
@@ -584,7 +647,7 @@ int tile_workers(size_t lanes, size_t prefixes, int sm_count) {
 struct Places { size_t offset, stat, acc, tile_lane, tile_prefix, tile_run, tile_stat, tile_acc, floats; };
 
 Places lane_places(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count) {
-    const Shape s = lane_shape(heads, head_width, sm_count);
+    const Shape s = lane_shape(heads, head_width, 4u, sm_count);      // workers go by the heads alone
     const size_t parts = (size_t)s.workers + lanes;
     const size_t workers = (size_t)tile_workers(lanes, prefixes, sm_count);
     const size_t rows = workers > 0 ? lanes * heads + workers * TILE : 0u;
@@ -607,15 +670,23 @@ Places lane_places(size_t lanes, size_t heads, size_t head_width, size_t prefixe
     return w;
 }
 
+// f(kernel) for the kernel of a head width.
+template <typename T, typename F>
+int with_rows_kernel(int lpr, bool full, F f) {
+    if (lpr == 8) return full ? f(k_lane_rows<T, 8, true>) : f(k_lane_rows<T, 8, false>);
+    if (lpr == 4) return full ? f(k_lane_rows<T, 4, true>) : f(k_lane_rows<T, 4, false>);
+    if (lpr == 2) return full ? f(k_lane_rows<T, 2, true>) : f(k_lane_rows<T, 2, false>);
+    return full ? f(k_lane_rows<T, 1, true>) : f(k_lane_rows<T, 1, false>);
+}
+size_t rows_smem(size_t lanes, const Shape &s) {
+    return ((lanes + 1u) * 4u + 15u) / 16u * 16u + (size_t)ROWS_DEPTH * 2u * (size_t)s.step * (size_t)s.row_pitch;
+}
 template <typename T>
 int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
-    const dim3 grid((unsigned)s.workers, (unsigned)s.groups), block((unsigned)(s.heads_per_cta * s.phases * 32));
-    const size_t smem = ((size_t)p.lanes + 1u) * sizeof(unsigned);
-    constexpr int U = sizeof(T) == 2 ? 2 : 1;
-    if (s.lpr == 8) return mb_launch(k_lane_rows<T, 8, U>, grid, block, smem, stream, p);
-    if (s.lpr == 4) return mb_launch(k_lane_rows<T, 4, U>, grid, block, smem, stream, p);
-    if (s.lpr == 2) return mb_launch(k_lane_rows<T, 2, U>, grid, block, smem, stream, p);
-    return mb_launch(k_lane_rows<T, 1, U>, grid, block, smem, stream, p);
+    const dim3 grid((unsigned)s.workers, (unsigned)s.groups), block((unsigned)((s.heads_per_cta * s.phases + 1) * 32));
+    return with_rows_kernel<T>(s.lpr, p.head_width == s.lpr * 16, [&](auto kernel) {
+        return mb_launch(kernel, grid, block, rows_smem((size_t)p.lanes, s), stream, p);
+    });
 }
 
 template <typename T, int SLABS>
@@ -624,7 +695,7 @@ size_t tile_smem(size_t lanes, size_t prefixes) {
 }
 template <typename T, int SLABS>
 int launch_tiles(const LaneP &p, cudaStream_t stream) {
-    return mb_launch(k_lane_prefix<T, SLABS>, dim3((unsigned)p.tile_workers), dim3(TILE), tile_smem<T, SLABS>((size_t)p.lanes, p.prefixes),
+    return mb_launch(k_lane_prefix<T, SLABS>, dim3((unsigned)p.tile_workers), dim3(TILE_THREADS), tile_smem<T, SLABS>((size_t)p.lanes, p.prefixes),
                      stream, p);
 }
 
@@ -656,7 +727,15 @@ extern "C" int mb_lane_attention_init(void) {
     const auto allow = [](auto kernel, size_t smem) {
         return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     };
-    int rc = allow(k_lane_prefix<float, 1>, tile_smem<float, 1>(MB_LANES_MAX, MB_LANES_MAX));
+    // a step of one phase may be above ROWS_STAGE: 12 heads of 128 f32 elements are 4 rows of 6 KB
+    constexpr size_t ROWS_SMEM_MOST = (MB_LANES_MAX + 4u) * 4u + ROWS_DEPTH * (ROWS_STAGE + 16u * 1024u);
+    int rc = 0;
+    for (int lpr = 1; lpr <= 8; lpr *= 2)
+        for (int full = 0; full < 2; ++full) {
+            if (rc == 0) rc = with_rows_kernel<float>(lpr, full, [&](auto k) { return allow(k, ROWS_SMEM_MOST); });
+            if (rc == 0) rc = with_rows_kernel<__half>(lpr, full, [&](auto k) { return allow(k, ROWS_SMEM_MOST); });
+        }
+    if (rc == 0) rc = allow(k_lane_prefix<float, 1>, tile_smem<float, 1>(MB_LANES_MAX, MB_LANES_MAX));
     if (rc == 0) rc = allow(k_lane_prefix<float, 2>, tile_smem<float, 2>(MB_LANES_MAX, MB_LANES_MAX));
     if (rc == 0) rc = allow(k_lane_prefix<__half, 1>, tile_smem<__half, 1>(MB_LANES_MAX, MB_LANES_MAX));
     if (rc == 0) rc = allow(k_lane_prefix<__half, 2>, tile_smem<__half, 2>(MB_LANES_MAX, MB_LANES_MAX));
@@ -664,7 +743,7 @@ extern "C" int mb_lane_attention_init(void) {
 }
 
 extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
-    const Shape s = lane_shape(a->heads, a->head_width, a->sm_count);
+    const Shape s = lane_shape(a->heads, a->head_width, a->cache.type == MB_F16 ? 2u : 4u, a->sm_count);
     const Places w = lane_places(a->lanes, a->heads, a->head_width, a->prefixes, a->sm_count);
     LaneP p = {};
     p.lanes = (int)a->lanes;
@@ -701,6 +780,9 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     p.acc = a->workspace + w.acc;
     p.heads_per_cta = s.heads_per_cta;
     p.phases = s.phases;
+    p.step = s.step;
+    p.row_bytes = s.row_bytes;
+    p.row_pitch = s.row_pitch;
     p.tile_workers = tile_workers(a->lanes, a->prefixes, a->sm_count);
     p.tile_lane = reinterpret_cast<unsigned *>(a->workspace + w.tile_lane);
     p.tile_prefix = reinterpret_cast<uint4 *>(a->workspace + w.tile_prefix);

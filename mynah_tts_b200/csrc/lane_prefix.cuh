@@ -11,9 +11,11 @@
 // (the others are below 2^-24 of the result).
 //
 // The blocks of all (tile, head) pairs, counted on, are cut into equal runs, one per CTA; a run
-// that ends inside a pair leaves a partial result, which k_lane_merge joins.  A thread owns a
-// row of the tile: its maximum, sum and weighted sum stay in registers, so tensor memory is never
-// rescaled.
+// that ends inside a pair leaves a partial result, which k_lane_merge joins.  Two threads own a
+// row of the tile, half of a block's scores and half of the columns each; its maximum, sum and
+// weighted sum stay in registers, so tensor memory is never rescaled.  The loops over scores and
+// pieces are kept rolled: most CTAs run through them a few times only, and unrolled code was
+// fetched at 200 cycles per score.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -22,8 +24,9 @@
 
 namespace {
 
-constexpr int TILE = 128;          // rows of a tile, threads of a CTA
-constexpr unsigned TILE_TMEM = 256, TILE_O = 128;   // columns; S and p below, O from there on
+constexpr int TILE = 128;          // rows of a tile
+constexpr int TILE_THREADS = 256;
+constexpr unsigned TILE_TMEM = 256, TILE_P = 128;   // columns: S, then O in its place, below; p from there on
 constexpr int TILE_CTAS_PER_SM = 2;
 
 template <typename T, int SLABS>
@@ -33,6 +36,8 @@ struct TileShape {
     static constexpr int QP = F16 ? 2 : 3, KP = F16 ? 1 : 3;   // planes of q and p, of K and V
     static constexpr int Q_SLAB = TILE * 128, K_SLAB = KEYS * 128;     // bytes of 64 columns
     static constexpr int Q_PLANE = SLABS * Q_SLAB, K_PLANE = SLABS * K_SLAB;
+    static constexpr int PIECES = KEYS * SLABS * 8 / TILE_THREADS;     // 8 elements of K and of V per thread
+    static constexpr int LOADS = F16 ? 1 : 2;                          // 16-byte loads of a piece
     static constexpr size_t SMEM = (size_t)QP * Q_PLANE + 2u * KP * K_PLANE + 1024u;
 };
 
@@ -56,15 +61,12 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
           "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
         :: "memory");
 }
-__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 // A from tensor memory, B from shared memory.
 __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
@@ -121,8 +123,26 @@ __device__ void tile_schedule(const LaneP &p, unsigned short *voice, unsigned *r
         voice[b] = w.prefix_rows > 0 ? (unsigned short)w.prefix : (unsigned short)0xffffu;
     }
     __syncthreads();
+    if (p.prefixes == 1) {             // all warps at once
+        __shared__ unsigned s_count[MB_LANES_MAX / 32];
+        const int warp = tid >> 5, chunks = (p.lanes + 31) / 32;
+        for (int c = warp; c < chunks; c += (int)blockDim.x >> 5) {
+            const int b = c * 32 + lane;
+            const unsigned has = __ballot_sync(MB_FULL, b < p.lanes && voice[b] == 0);
+            if (lane == 0) s_count[c] = __popc(has);
+            if (b < p.lanes) rank[b] = has >> lane & 1u ? (unsigned)__popc(has & ((1u << lane) - 1u)) : 0xffffffffu;
+        }
+        __syncthreads();
+        for (int c = warp; c < chunks; c += (int)blockDim.x >> 5) {
+            const unsigned before = __reduce_add_sync(MB_FULL, lane < c ? s_count[lane] : 0u);
+            const int b = c * 32 + lane;
+            if (b < p.lanes && rank[b] != 0xffffffffu) rank[b] += before;
+            if (c == chunks - 1 && lane == 0) prefix[0].z = before + s_count[c];
+        }
+        __syncthreads();
+    }
     if (tid < 32) {
-        for (int b0 = 0; b0 < p.lanes; b0 += 32) {
+        for (int b0 = 0; b0 < p.lanes && p.prefixes > 1; b0 += 32) {
             const int b = b0 + lane;
             const unsigned g = b < p.lanes ? voice[b] : 0xffffu;
             const unsigned peers = __match_any_sync(MB_FULL, g);
@@ -158,28 +178,30 @@ __device__ void tile_schedule(const LaneP &p, unsigned short *voice, unsigned *r
 }
 
 template <typename T, int SLABS>
-__global__ void __launch_bounds__(TILE, TILE_CTAS_PER_SM) k_lane_prefix(LaneP p) {
+__global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 1) k_lane_prefix(LaneP p) {
     using C = TileShape<T, SLABS>;
     constexpr bool F16 = C::F16;
-    constexpr int KEYS = C::KEYS, QP = C::QP, KP = C::KP;
+    constexpr int KEYS = C::KEYS, QP = C::QP, KP = C::KP, PIECES = C::PIECES, LOADS = C::LOADS;
+    constexpr int HALF = KEYS / 2, COLS = SLABS * 32;      // scores and columns of a thread
     extern __shared__ unsigned char sm_tile[];
     __shared__ __align__(8) unsigned long long s_bar;
     __shared__ uint32_t s_tmem;
     __shared__ unsigned s_units, s_run;
     __shared__ unsigned short s_row[TILE];                 // lanes of the tile
+    __shared__ float s_unscale[TILE], s_half[2][TILE];
     unsigned char *base = sm_tile + ((1024u - (saddr(sm_tile) & 1023u)) & 1023u);
     unsigned char *sq = base, *sk = sq + QP * C::Q_PLANE, *sv = sk + KP * C::K_PLANE;
     unsigned char *rest = base + (C::SMEM - 1024u);        // schedule
     uint4 *s_prefix = reinterpret_cast<uint4 *>(rest);
     unsigned *s_rank = reinterpret_cast<unsigned *>(s_prefix + p.prefixes);
     unsigned short *s_voice = reinterpret_cast<unsigned short *>(s_rank + p.lanes);
-    const int tid = threadIdx.x, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = tid % TILE, half = tid / TILE;
     mb_pdl_wait();
     mb_pdl_trigger();
     tile_schedule<KEYS>(p, s_voice, s_rank, s_prefix, &s_units, &s_run);
     if (blockIdx.x == 0) {
-        for (int b = tid; b < p.lanes; b += TILE) p.tile_lane[b] = s_rank[b];
-        for (int g = tid; g < (int)p.prefixes; g += TILE) p.tile_prefix[g] = s_prefix[g];
+        for (int b = tid; b < p.lanes; b += TILE_THREADS) p.tile_lane[b] = s_rank[b];
+        for (int g = tid; g < (int)p.prefixes; g += TILE_THREADS) p.tile_prefix[g] = s_prefix[g];
         if (tid == 0) *p.tile_run = s_run;
     }
     const unsigned units = s_units, run = s_run;
@@ -197,11 +219,11 @@ __global__ void __launch_bounds__(TILE, TILE_CTAS_PER_SM) k_lane_prefix(LaneP p)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = s_tmem, my_tmem = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t tmem = s_tmem, my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16);    // a warp reaches 32 rows
     const int hw = p.head_width, ksteps = (hw + 15) / 16, ncols = ksteps * 16;
     const uint32_t format = F16 ? 0u : (1u << 7 | 1u << 10);
     const uint32_t idesc_s = instr_desc_f16(TILE, KEYS) | format;
-    const uint32_t idesc_o = instr_desc_f16(TILE, ncols) | format | 1u << 16;          // B along N
+    const uint32_t idesc_o = instr_desc_f16(TILE, ncols) | format | 1u << 16;              // B along N
     unsigned parity = 0;
     bool fine = true;
     int g = 0;
@@ -216,90 +238,104 @@ __global__ void __launch_bounds__(TILE, TILE_CTAS_PER_SM) k_lane_prefix(LaneP p)
         const int rows = (int)min((unsigned)TILE, of.z - tile * TILE);
         const unsigned keys = min(p.prefix_length[g], p.prefix_capacity);
         unit += stop - block;
-        __syncthreads();                                   // s_row, and the operands of the last block
-        for (int b = tid; b < p.lanes; b += TILE)
+
+        // K and V rows of a block on their way, zero beyond the prefix and beyond the head (rows
+        // that are not seen may hold anything)
+        const size_t origin = (size_t)g * p.prefix_stride + (size_t)head * hw;
+        const T *pk = reinterpret_cast<const T *>(p.prefix_k) + origin, *pv = reinterpret_cast<const T *>(p.prefix_v) + origin;
+        uint4 kx[PIECES][LOADS], vx[PIECES][LOADS];
+        auto fetch = [&](unsigned block) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int at = tid + i * TILE_THREADS, r = at / (SLABS * 8), d = at % (SLABS * 8) * 8;
+                const unsigned j = block * KEYS + r;
+#pragma unroll
+                for (int l = 0; l < LOADS; ++l) {
+                    kx[i][l] = vx[i][l] = make_uint4(0, 0, 0, 0);
+                    if (j < keys && d + 4 * l < hw) {
+                        const size_t from = (size_t)j * p.prefix_row_stride + d + 4 * l;
+                        kx[i][l] = __ldg(reinterpret_cast<const uint4 *>(pk + from));
+                        vx[i][l] = __ldg(reinterpret_cast<const uint4 *>(pv + from));
+                    }
+                }
+            }
+        };
+        fetch(block);
+        __syncthreads();                                   // s_row
+        for (int b = tid; b < p.lanes; b += TILE_THREADS)
             if (s_voice[b] == g && s_rank[b] / TILE == tile) s_row[s_rank[b] % TILE] = (unsigned short)b;
         __syncthreads();
 
-        // this thread's query: scaled, cut into planes, rows of 128 bytes per slab
-        const bool mine = tid < rows;
-        unsigned seen_head = 0, seen_from = 0;             // rows of the prefix it sees: below, and from there on
-        float unscale = 1.0f;
-        {
-            const int b = mine ? s_row[tid] : 0;
-            const float *q = p.qkv + (size_t)b * p.qkv_stride + head * hw;
-            float up = 1.0f;
-            if (mine) {
-                const LaneView w = lane_view(p, b);
-                seen_head = w.prefix_head;
-                seen_from = w.prefix_head + w.prefix_jump;
+        // the queries: scaled, cut into planes, rows of 128 bytes per slab
+        constexpr int PER_ROW = SLABS * 8, QUERIES = 4;
+#pragma unroll 1
+        for (int i0 = tid; i0 - lane < rows * PER_ROW; i0 += QUERIES * TILE_THREADS) {
+            float x[QUERIES][8];
+#pragma unroll
+            for (int u = 0; u < QUERIES; ++u) {
+                const int i = i0 + u * TILE_THREADS, r = i / PER_ROW, c = i % PER_ROW;
+                const float *q = p.qkv + (size_t)(r < rows ? s_row[r] : 0) * p.qkv_stride + head * hw + c * 8;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[u][j] = r < rows && c * 8 + j < hw ? q[j] * p.scale_log2 : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < QUERIES; ++u) {
+                const int i = i0 + u * TILE_THREADS, r = i / PER_ROW, c = i % PER_ROW;
+                float most = 0.0f, up = 1.0f, down = 1.0f;
                 if (F16) {
-                    float most = 0.0f;
-                    for (int d = 0; d < hw; ++d) most = fmaxf(most, fabsf(q[d] * p.scale_log2));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[u][j]));
+#pragma unroll
+                    for (int o = PER_ROW / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(MB_FULL, most, o));
                     // 2^e <= most < 2^(e + 1); zero and what is not finite stay as they are
                     const int e = (int)(__float_as_uint(most) >> 23) - 127;
                     if (e > -126 && e < 127) {
                         up = __uint_as_float((unsigned)(127 - e) << 23);
-                        unscale = __uint_as_float((unsigned)(127 + e) << 23);
+                        down = __uint_as_float((unsigned)(127 + e) << 23);
                     }
                 }
-            }
+                if (r < rows) {
+                    uint32_t plane[4][QP];
 #pragma unroll
-            for (int c = 0; c < SLABS * 8; ++c) {
-                uint32_t plane[4][QP];
+                    for (int j = 0; j < 4; ++j) split_pair<F16>(x[u][2 * j] * up, x[u][2 * j + 1] * up, plane[j]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = c * 8 + 2 * i;
-                    const float x = mine && d < hw ? q[d] * p.scale_log2 * up : 0.0f;
-                    const float y = mine && d + 1 < hw ? q[d + 1] * p.scale_log2 * up : 0.0f;
-                    split_pair<F16>(x, y, plane[i]);
+                    for (int j = 0; j < QP; ++j)
+                        *reinterpret_cast<uint4 *>(sq + j * C::Q_PLANE + (c >> 3) * C::Q_SLAB + swizzled(r, c & 7)) =
+                            make_uint4(plane[0][j], plane[1][j], plane[2][j], plane[3][j]);
+                    if (c == 0) s_unscale[r] = down;
                 }
-#pragma unroll
-                for (int j = 0; j < QP; ++j)
-                    *reinterpret_cast<uint4 *>(sq + j * C::Q_PLANE + (c >> 3) * C::Q_SLAB + swizzled(tid, c & 7)) =
-                        make_uint4(plane[0][j], plane[1][j], plane[2][j], plane[3][j]);
             }
         }
-        float top = -INFINITY, sum = 0.0f, o[SLABS * 64];
+        const bool mine = row < rows;
+        const bool work = (warp & 3) * 32 < rows;          // a warp without a row has nothing to weigh
+        unsigned seen_head = 0, seen_from = 0;             // rows of the prefix it sees: below, and from there on
+        if (mine) {
+            const LaneView w = lane_view(p, s_row[row]);
+            seen_head = w.prefix_head;
+            seen_from = w.prefix_head + w.prefix_jump;
+        }
+        float unscale = 1.0f, top = -INFINITY, sum = 0.0f, o[COLS];
 #pragma unroll
-        for (int i = 0; i < SLABS * 64; ++i) o[i] = 0.0f;
+        for (int i = 0; i < COLS; ++i) o[i] = 0.0f;
 
-        for (; block < stop; ++block) {
+        for (bool begun = false; block < stop; ++block, begun = true) {
             const unsigned first = block * KEYS;
-            // K and V rows, zero beyond the prefix and beyond the head (unseen rows may hold anything)
-            const size_t origin = (size_t)g * p.prefix_stride + (size_t)head * hw;
-            const T *pk = reinterpret_cast<const T *>(p.prefix_k) + origin, *pv = reinterpret_cast<const T *>(p.prefix_v) + origin;
-#pragma unroll 4
-            for (int i = tid; i < KEYS * SLABS * 8; i += TILE) {
-                const int r = i / (SLABS * 8), c = i % (SLABS * 8), d = c * 8;
-                const bool in = first + r < keys;
-                const size_t at = (size_t)(first + r) * p.prefix_row_stride + d;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int at = tid + i * TILE_THREADS, r = at / (SLABS * 8), c = at % (SLABS * 8);
                 const unsigned to = (c >> 3) * C::K_SLAB + swizzled(r, c & 7);
                 if (F16) {
-                    uint4 x = make_uint4(0, 0, 0, 0), y = x;
-                    if (in && d < hw) {
-                        x = __ldg(reinterpret_cast<const uint4 *>(pk + at));
-                        y = __ldg(reinterpret_cast<const uint4 *>(pv + at));
-                    }
-                    *reinterpret_cast<uint4 *>(sk + to) = x;
-                    *reinterpret_cast<uint4 *>(sv + to) = y;
+                    *reinterpret_cast<uint4 *>(sk + to) = kx[i][0];
+                    *reinterpret_cast<uint4 *>(sv + to) = vx[i][0];
                 } else {
-                    float4 x[4];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        x[j] = x[2 + j] = make_float4(0, 0, 0, 0);
-                        if (in && d + 4 * j < hw) {
-                            x[j] = __ldg(reinterpret_cast<const float4 *>(pk + at + 4 * j));
-                            x[2 + j] = __ldg(reinterpret_cast<const float4 *>(pv + at + 4 * j));
-                        }
-                    }
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
+                        const uint4 a = m ? vx[i][0] : kx[i][0], b = m ? vx[i][LOADS - 1] : kx[i][LOADS - 1];
                         uint32_t plane[4][KP];
-                        split_pair<F16>(x[2 * m].x, x[2 * m].y, plane[0]);
-                        split_pair<F16>(x[2 * m].z, x[2 * m].w, plane[1]);
-                        split_pair<F16>(x[2 * m + 1].x, x[2 * m + 1].y, plane[2]);
-                        split_pair<F16>(x[2 * m + 1].z, x[2 * m + 1].w, plane[3]);
+                        split_pair<F16>(__uint_as_float(a.x), __uint_as_float(a.y), plane[0]);
+                        split_pair<F16>(__uint_as_float(a.z), __uint_as_float(a.w), plane[1]);
+                        split_pair<F16>(__uint_as_float(b.x), __uint_as_float(b.y), plane[2]);
+                        split_pair<F16>(__uint_as_float(b.z), __uint_as_float(b.w), plane[3]);
 #pragma unroll
                         for (int j = 0; j < KP; ++j)
                             *reinterpret_cast<uint4 *>((m ? sv : sk) + j * C::K_PLANE + to) =
@@ -312,61 +348,75 @@ __global__ void __launch_bounds__(TILE, TILE_CTAS_PER_SM) k_lane_prefix(LaneP p)
             __syncthreads();
             if (tid == 0) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t more = 0u;
+                const uint64_t dq = smem_desc_sw128(saddr(sq)), dk = smem_desc_sw128(saddr(sk));
 #pragma unroll
-                for (int a = 0; a < QP; ++a)
+                for (int s = 0; s < SLABS * 4; ++s) {
+                    if (s >= ksteps) break;
+                    const unsigned off = (unsigned)(s & 3) * 2u;           // 16 columns, in 16-byte units
 #pragma unroll
-                    for (int b = 0; b < KP; ++b) {
-                        if (!F16 && a + b > 2) continue;
-                        for (int s = 0; s < ksteps; ++s) {
-                            const unsigned slab = s >> 2, off = (s & 3) * 32u;
-                            mma_f16(tmem, smem_desc_sw128(saddr(sq) + a * C::Q_PLANE + slab * C::Q_SLAB + off),
-                                    smem_desc_sw128(saddr(sk) + b * C::K_PLANE + slab * C::K_SLAB + off), idesc_s, more);
-                            more = 1u;
+                    for (int a = 0; a < QP; ++a)
+#pragma unroll
+                        for (int b = 0; b < KP; ++b) {
+                            if (!F16 && a + b > 2) continue;
+                            mma_f16(tmem, dq + (a * C::Q_PLANE + (s >> 2) * C::Q_SLAB) / 16 + off,
+                                    dk + (b * C::K_PLANE + (s >> 2) * C::K_SLAB) / 16 + off, idesc_s, s + a + b > 0);
                         }
-                    }
+                }
                 mma_commit(&s_bar);
             }
+            if (block + 1 < stop) fetch(block + 1);
+            if (!begun) unscale = mine ? s_unscale[row] : 1.0f;
             bool done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
             parity ^= 1u;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float keep = 1.0f;
-            if (done && warp * 32 < rows) {                // a warp without a row has nothing to weigh
-                uint32_t x[KEYS / 32][32];
+            // masked: beyond the prefix, or between the first rows and the window
+            const bool all = first + KEYS <= keys && (first + KEYS <= seen_head || first >= seen_from);
+            uint32_t x[32];
+            auto scores = [&](int i) {
+                tmem_ld32u(my_tmem + half * HALF + i * 32, x);
+                tmem_ld_wait(x);
+                if (!__all_sync(MB_FULL, all)) {
 #pragma unroll
-                for (int i = 0; i < KEYS / 32; ++i) tmem_ld32u(my_tmem + i * 32, x[i]);
-#pragma unroll
-                for (int i = 0; i < KEYS / 32; ++i) tmem_ld_wait(x[i]);
-                // masked: beyond the prefix, or between the first rows and the window
-                const bool all = first + KEYS <= keys && (first + KEYS <= seen_head || first >= seen_from);
-                float m = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < KEYS; ++i) {
-                    const unsigned j = first + i;
-                    if (!all && !(j < keys && (j < seen_head || j >= seen_from))) x[i / 32][i % 32] = 0xff800000u;
-                    m = fmaxf(m, __uint_as_float(x[i / 32][i % 32]));
+                    for (int k = 0; k < 32; ++k) {
+                        const unsigned j = first + half * HALF + i * 32 + k;
+                        if (!(j < keys && (j < seen_head || j >= seen_from))) x[k] = 0xff800000u;
+                    }
                 }
-                m = fmaxf(top, m * unscale);
+            };
+            float m = -INFINITY;
+            if (done && work) {
+#pragma unroll 1
+                for (int i = 0; i < HALF / 32; ++i) {
+                    scores(i);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) m = fmaxf(m, __uint_as_float(x[k]));
+                }
+                s_half[half][row] = m;
+            }
+            __syncthreads();
+            float keep = 1.0f;
+            if (done && work) {
+                m = fmaxf(top, fmaxf(m, s_half[half ^ 1][row]) * unscale);
                 const float ref = m == -INFINITY ? 0.0f : m;
                 keep = pow2(top - ref);
                 top = m;
                 sum *= keep;
+#pragma unroll 1
+                for (int i = 0; i < HALF / 32; ++i) {
+                    if (HALF > 32) scores(i);              // one group: still there
+                    uint32_t out[QP][16];
 #pragma unroll
-                for (int i = 0; i < KEYS / 64; ++i) {
-                    uint32_t out[QP][32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int k = i * 64 + 2 * j;
-                        const float a = pow2(fmaf(__uint_as_float(x[k / 32][k % 32]), unscale, -ref));
-                        const float b = pow2(fmaf(__uint_as_float(x[(k + 1) / 32][(k + 1) % 32]), unscale, -ref));
+                    for (int k = 0; k < 16; ++k) {
+                        const float a = pow2(fmaf(__uint_as_float(x[2 * k]), unscale, -ref));
+                        const float b = pow2(fmaf(__uint_as_float(x[2 * k + 1]), unscale, -ref));
                         sum += a + b;
                         uint32_t plane[QP];
                         split_pair<F16>(a, b, plane);
 #pragma unroll
-                        for (int l = 0; l < QP; ++l) out[l][j] = plane[l];
+                        for (int l = 0; l < QP; ++l) out[l][k] = plane[l];
                     }
 #pragma unroll
-                    for (int l = 0; l < QP; ++l) tmem_st32u(my_tmem + l * (KEYS / 2) + i * 32, out[l]);
+                    for (int l = 0; l < QP; ++l) tmem_st16u(my_tmem + TILE_P + l * HALF + half * (HALF / 2) + i * 16, out[l]);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
@@ -375,45 +425,47 @@ __global__ void __launch_bounds__(TILE, TILE_CTAS_PER_SM) k_lane_prefix(LaneP p)
             if (!fine) break;
             if (tid == 0) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t more = 0u;
+                const uint64_t dv = smem_desc_sw128_mn(saddr(sv), C::K_SLAB);
 #pragma unroll
-                for (int a = 0; a < QP; ++a)
+                for (int s = 0; s < KEYS / 16; ++s)
 #pragma unroll
-                    for (int b = 0; b < KP; ++b) {
-                        if (!F16 && a + b > 2) continue;
+                    for (int a = 0; a < QP; ++a)
 #pragma unroll
-                        for (int s = 0; s < KEYS / 16; ++s) {
-                            mma_f16_ts(tmem + TILE_O, tmem + a * (KEYS / 2) + s * 8,
-                                       smem_desc_sw128_mn(saddr(sv) + b * C::K_PLANE + s * 2048u, C::K_SLAB), idesc_o, more);
-                            more = 1u;
+                        for (int b = 0; b < KP; ++b) {
+                            if (!F16 && a + b > 2) continue;
+                            mma_f16_ts(tmem, tmem + TILE_P + a * HALF + s * 8, dv + (b * C::K_PLANE + s * 2048) / 16, idesc_o,
+                                       s + a + b > 0);
                         }
-                    }
                 mma_commit(&s_bar);
             }
             done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
             parity ^= 1u;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (done && warp * 32 < rows) {
+            if (done && work) {
 #pragma unroll
-                for (int i = 0; i < SLABS * 2; ++i) {
-                    if (i * 32 >= ncols) break;
-                    uint32_t x[32];
-                    tmem_ld32u(my_tmem + TILE_O + i * 32, x);
+                for (int i = 0; i < SLABS; ++i) {
+                    if (half * COLS + i * 32 >= ncols) break;
+                    tmem_ld32u(my_tmem + half * COLS + i * 32, x);
                     tmem_ld_wait(x);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[i * 32 + j] = fmaf(o[i * 32 + j], keep, __uint_as_float(x[j]));
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            fine = __syncthreads_and(done);
+            fine = __syncthreads_and(done);                // before S and the operands are written again
             if (!fine) break;
         }
-        if (mine && fine) {
-            const size_t at = of.y + (size_t)tile * TILE * p.heads + (size_t)head * rows + (size_t)blockIdx.x * TILE + tid;
-            p.tile_stat[at] = make_float2(top, sum);
+        if (fine) {
+            if (half == 1) s_half[0][row] = sum;
+            __syncthreads();
+            if (mine) {
+                const size_t at = of.y + (size_t)tile * TILE * p.heads + (size_t)head * rows + (size_t)blockIdx.x * TILE + row;
+                if (half == 0) p.tile_stat[at] = make_float2(top, sum + s_half[0][row]);
 #pragma unroll
-            for (int i = 0; i < SLABS * 64; i += 4)
-                if (i < hw) *reinterpret_cast<float4 *>(p.tile_acc + at * hw + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int i = 0; i < COLS; i += 4)
+                    if (half * COLS + i < hw)
+                        *reinterpret_cast<float4 *>(p.tile_acc + at * hw + half * COLS + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
         }
     }
     if (!fine && tid == 0) {
