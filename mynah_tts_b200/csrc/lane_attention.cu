@@ -67,13 +67,23 @@ struct LaneView {
     bool ok;
 };
 
-__device__ __forceinline__ LaneView lane_view(const LaneP &p, int b) {
+// The words it is made of, loaded side by side.
+struct LaneWords { unsigned live, slot, length, prefix; };
+
+__device__ __forceinline__ LaneWords lane_words(const LaneP &p, int b) {
+    LaneWords x;
+    x.live = p.live != nullptr ? *p.live : 0xffffffffu;
+    x.slot = p.slot != nullptr ? p.slot[b] : (unsigned)b;
+    x.length = p.length[b];
+    x.prefix = p.prefixes == 0 ? 0u : p.lane_prefix != nullptr ? p.lane_prefix[b] : 0u;
+    return x;
+}
+__device__ __forceinline__ LaneView lane_view(const LaneP &p, int b, const LaneWords &x) {
     LaneView w;
-    const unsigned live = p.live != nullptr ? *p.live : 0xffffffffu;
-    w.ok = (unsigned)b < live;
-    w.slot = p.slot != nullptr ? p.slot[b] : (unsigned)b;
-    const unsigned n = p.length[b];
-    w.prefix = p.prefixes == 0 ? 0u : p.lane_prefix != nullptr ? p.lane_prefix[b] : 0u;
+    w.ok = (unsigned)b < x.live;
+    w.slot = x.slot;
+    w.prefix = x.prefix;
+    const unsigned n = x.length;
     const unsigned P = w.prefix < p.prefixes ? min(p.prefix_length[w.prefix], p.prefix_capacity) : 0u;
     if (w.slot >= p.slots || (p.window == 0 && n >= p.capacity)) w.ok = false;
     w.keep = 0;
@@ -103,6 +113,8 @@ __device__ __forceinline__ LaneView lane_view(const LaneP &p, int b) {
     if (!w.ok) w.prefix_rows = w.own_rows = 0;
     return w;
 }
+__device__ __forceinline__ LaneView lane_view(const LaneP &p, int b) { return lane_view(p, b, lane_words(p, b)); }
+
 __device__ __forceinline__ unsigned own_row(const LaneP &p, const LaneView &w, unsigned i) {
     if (i < w.own_head) return i;
     const unsigned r = w.own_base + (i - w.own_head);
@@ -226,7 +238,7 @@ __device__ __forceinline__ void bar_arrive(void *bar) {
 
 // FULL: the head fills all columns, LPR * 16.
 template <typename T, int LPR, bool FULL>
-__global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows(LaneP p) {
+__global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
     extern __shared__ uint4 sm_rows_dyn[];
     __shared__ unsigned s_run;
     __shared__ float s_acc[WARPS_MAX][MB_LANE_HEAD_WIDTH_MAX];
@@ -244,8 +256,13 @@ __global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    mb_pdl_wait();
+    // Behind k_lane_prefix, which began when all work before it had ended, nothing has to be waited
+    // for: both run side by side, and this one ends after the other (last_wait).
+    if (p.tile_workers == 0) mb_pdl_wait();
     mb_pdl_trigger();
+    const auto last_wait = [&]() {
+        if (p.tile_workers > 0) mb_pdl_wait();
+    };
     lane_schedule(p, sm_off, &s_run, gridDim.x, GROUPS * p.phases);
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         for (int i = threadIdx.x; i <= p.lanes; i += blockDim.x) p.offset[i] = sm_off[i];
@@ -253,7 +270,7 @@ __global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows
     }
     const unsigned total = sm_off[p.lanes], run = s_run;
     const unsigned long long begin = (unsigned long long)blockIdx.x * run;
-    if (begin >= total) return;
+    if (begin >= total) { last_wait(); return; }
     const unsigned end = (unsigned)min((unsigned long long)total, begin + run);
     unsigned at = (unsigned)begin;
     int b = 0;                                   // the lane that row `at` belongs to
@@ -297,6 +314,7 @@ __global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows
             }
         }
         if (!fine && lane == 0) atomicOr(p.status, 2);
+        last_wait();
         return;
     }
 
@@ -317,8 +335,9 @@ __global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows
         }
         for (unsigned r0 = first; r0 < last; r0 += step) {
             const bool there = __all_sync(MB_FULL, bar_wait(&s_full[stage], parity, TC_SPIN));
-            if (!there) {                        // what is still on its way gets no second chance to be waited for: TC_SPIN is seconds
+            if (!there) {                        // the wait has lasted seconds: nothing can be on its way any more
                 if (lane == 0) atomicOr(p.status, 2);
+                last_wait();
                 return;
             }
             const char *from = mine + (size_t)stage * 2u * plane;
@@ -424,6 +443,7 @@ __global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows
         at += last - first;
         ++b;
     }
+    last_wait();
 }
 
 }  // namespace
@@ -432,10 +452,11 @@ __global__ void __launch_bounds__((WARPS_MAX + 1) * 32, CTAS_PER_SM) k_lane_rows
 
 namespace {
 
-// One CTA per head of a lane: the new row's score, the lane's partials, the result, and the new
-// row into the cache.  Four columns per thread, threads of the same columns take every
-// SLICES-th partial, MERGE_U at a time (a lane alone has hundreds).  A lane whose cache is full
-// or whose slot does not exist is left out and sets the status word.
+// The new row's score, a lane's partials, the result, and the new row into the cache, for one
+// head by `warps` warps: one where there are many heads of lanes, sixteen where there are few (a
+// lane alone has hundreds of partials).  Four columns per thread; threads of the same columns take
+// every slices-th partial, MERGE_U at a time.  A lane whose cache is full or whose slot does not
+// exist is left out and sets the status word.
 constexpr int MERGE_U = 4;
 
 struct Merged { float top, sum; float4 acc; };
@@ -445,9 +466,10 @@ __device__ __forceinline__ void add4(float4 &a, const float4 &b, float f) {
     a.x = fmaf(b.x, f, a.x); a.y = fmaf(b.y, f, a.y); a.z = fmaf(b.z, f, a.z); a.w = fmaf(b.w, f, a.w);
 }
 
-// Joins the slices of a CTA; the result is in the first `columns` threads.
+// Joins the slices of a head; the result is in the first `columns` threads of its first warp.
+template <int WARPS>
 __device__ __forceinline__ Merged join_slices(Merged r, int columns, float4 (*s_acc)[32], float2 *s_stat) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float m = r.top;
     for (int o = columns; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(MB_FULL, m, o));
     const float f = pow2(r.top - (m == -INFINITY ? 0.0f : m));
@@ -460,16 +482,17 @@ __device__ __forceinline__ Merged join_slices(Merged r, int columns, float4 (*s_
         r.acc.z += __shfl_xor_sync(MB_FULL, r.acc.z, o);
         r.acc.w += __shfl_xor_sync(MB_FULL, r.acc.w, o);
     }
+    r.top = m;
+    if (WARPS == 1) return r;
     if (lane < columns) s_acc[warp][lane] = r.acc;
     if (lane == 0) s_stat[warp] = make_float2(m, r.sum);
     __syncthreads();
-    r.top = m;
     if (warp != 0 || lane >= columns) return r;
-    for (int o = 1; o < warps; ++o) r.top = fmaxf(r.top, s_stat[o].x);
+    for (int o = 1; o < WARPS; ++o) r.top = fmaxf(r.top, s_stat[o].x);
     const float ref = r.top == -INFINITY ? 0.0f : r.top;
     r.sum = 0.0f;
     r.acc = make_float4(0, 0, 0, 0);
-    for (int o = 0; o < warps; ++o) {
+    for (int o = 0; o < WARPS; ++o) {
         const float g = pow2(s_stat[o].x - ref);
         r.sum = fmaf(s_stat[o].y, g, r.sum);
         add4(r.acc, s_acc[o][lane], g);
@@ -477,37 +500,49 @@ __device__ __forceinline__ Merged join_slices(Merged r, int columns, float4 (*s_
     return r;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
-    __shared__ float4 s_acc[16][32];
-    __shared__ float2 s_stat[16];
+constexpr int MERGE_HEADS = 4;     // heads of a CTA with one warp each
+
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? MERGE_HEADS * 32 : WARPS * 32) k_lane_merge(LaneP p, int columns) {
+    __shared__ float4 s_acc[WARPS == 1 ? 1 : WARPS][32];
+    __shared__ float2 s_stat[WARPS];
     __shared__ int s_again;
-    const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
-    // lane state and rows were written before the first kernel of the call began
-    if (p.live != nullptr && (unsigned)b >= *p.live) return;
-    const LaneView w = lane_view(p, b);
-    const int column = tid % columns, slice = tid / columns, slices = blockDim.x / columns;
+    const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = WARPS == 1 ? (int)blockIdx.y * MERGE_HEADS + warp : (int)blockIdx.y, tid = WARPS == 1 ? lane : (int)threadIdx.x;
+    if (head >= p.heads) return;       // a warp of its own
+    const int column = tid % columns, slice = tid / columns, slices = WARPS * 32 / columns;
     const int d = column * 4;
     const bool mine = d < p.head_width;
+    // written before the first kernel of the call began: on their way while this one waits
+    const LaneWords words = lane_words(p, b);
     const float *row = p.qkv + (size_t)b * p.qkv_stride + head * p.head_width + d;
-    T kt[4], vt[4];
-    float q[4], x = 0.0f;
+    float q[4], kf[4], vf[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        kt[i] = (T)(mine ? row[p.width + i] : 0.0f);
-        vt[i] = (T)(mine ? row[2 * p.width + i] : 0.0f);
-        q[i] = mine ? row[i] * p.scale_log2 : 0.0f;
-        x = fmaf(q[i], (float)kt[i], x);
+        q[i] = mine ? row[i] : 0.0f;
+        kf[i] = mine ? row[p.width + i] : 0.0f;
+        vf[i] = mine ? row[2 * p.width + i] : 0.0f;
     }
-    for (int o = columns >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(MB_FULL, x, o);
-    if (tid == 0) s_again = 0;
+    if (threadIdx.x == 0) s_again = 0;
     mb_pdl_wait();
     mb_pdl_trigger();
+    const unsigned first = p.offset[b], last = p.offset[b + 1], run = p.offset[p.lanes + 1];
+    if ((unsigned)b >= words.live) return;
+    const LaneView w = lane_view(p, b, words);
     if (!w.ok) {
         if (tid == 0 && head == 0) atomicOr(p.status, 32);
         return;
     }
-    const unsigned first = p.offset[b], last = p.offset[b + 1], run = p.offset[p.lanes + 1];
+    T kt[4], vt[4];
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        kt[i] = (T)kf[i];
+        vt[i] = (T)vf[i];
+        q[i] *= p.scale_log2;
+        x = fmaf(q[i], (float)kt[i], x);
+    }
+    for (int o = columns >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(MB_FULL, x, o);
     const unsigned part0 = last > first ? first / run : 0u;
     const int n_rows = last > first ? (int)((last - 1) / run - part0) + 1 : 0;
     const size_t base = (size_t)(part0 + b) * p.heads + head;
@@ -541,14 +576,11 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
             const int i = i0 + u * slices;
             s[u] = make_float2(-INFINITY, 0.0f);
             a[u] = make_float4(0, 0, 0, 0);
-            if (i < n_rows) {
-                const size_t at = base + (size_t)i * p.heads;
-                s[u] = p.stat[at];
-                if (mine) a[u] = *reinterpret_cast<const float4 *>(p.acc + at * p.head_width + d);
-            } else if (i < n) {
-                const size_t at = tile_base + (size_t)(i - n_rows) * TILE;
-                s[u] = p.tile_stat[at];
-                if (mine) a[u] = *reinterpret_cast<const float4 *>(p.tile_acc + at * p.head_width + d);
+            if (i < n) {
+                const bool tile = i >= n_rows;
+                const size_t at = tile ? tile_base + (size_t)(i - n_rows) * TILE : base + (size_t)i * p.heads;
+                s[u] = (tile ? p.tile_stat : p.stat)[at];
+                if (mine) a[u] = *reinterpret_cast<const float4 *>((tile ? p.tile_acc : p.acc) + at * p.head_width + d);
             }
         }
         float m = r.top;
@@ -565,7 +597,7 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
             add4(r.acc, a[u], f);
         }
     }
-    r = join_slices(r, columns, s_acc, s_stat);
+    r = join_slices<WARPS>(r, columns, s_acc, s_stat);
     float *out = p.out + (size_t)b * p.out_stride + head * p.head_width + d;
     auto store = [&]() {
         const float y[4] = {__fdiv_rn(r.acc.x, r.sum), __fdiv_rn(r.acc.y, r.sum), __fdiv_rn(r.acc.z, r.sum), __fdiv_rn(r.acc.w, r.sum)};
@@ -578,10 +610,15 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
         return finite;
     };
     const bool stores = tid < columns && mine;
-    if (stores && !store() && p.tile_workers > 0) s_again = 1;
+    const bool odd = stores && !store();
     if (p.tile_workers == 0) return;
-    __syncthreads();
-    if (s_again == 0) return;
+    if (WARPS == 1) {
+        if (!__any_sync(MB_FULL, odd)) return;
+    } else {
+        if (odd) s_again = 1;
+        __syncthreads();
+        if (s_again == 0) return;
+    }
     // Infinities or NaN among the rows: a value kept as planes turns inf into inf - inf, so this
     // head is formed once more from the values themselves, row by row.
     const size_t prefix = (size_t)w.prefix * p.prefix_stride + head * p.head_width + d;
@@ -613,7 +650,7 @@ __global__ void __launch_bounds__(512) k_lane_merge(LaneP p, int columns) {
         scale4(r.acc, keep);
         if (in) add4(r.acc, make_float4(vx[0], vx[1], vx[2], vx[3]), e);
     }
-    r = join_slices(r, columns, s_acc, s_stat);
+    r = join_slices<WARPS>(r, columns, s_acc, s_stat);
     if (stores) store();
 }
 
@@ -640,7 +677,7 @@ Shape lane_shape(size_t heads, size_t head_width, size_t size, int sm_count) {
 constexpr size_t TILE_LANES = 16;
 
 int tile_workers(size_t lanes, size_t prefixes, int sm_count) {
-    return prefixes > 0 && lanes >= TILE_LANES ? TILE_CTAS_PER_SM * sm_count : 0;
+    return prefixes > 0 && lanes >= TILE_LANES ? sm_count : 0;      // one CTA per SM beside one of k_lane_rows
 }
 
 // Places of the workspace, in floats.
@@ -683,15 +720,22 @@ size_t rows_smem(size_t lanes, const Shape &s) {
 }
 template <typename T>
 int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
-    const dim3 grid((unsigned)s.workers, (unsigned)s.groups), block((unsigned)((s.heads_per_cta * s.phases + 1) * 32));
+    // beside k_lane_prefix an SM has room for one CTA; runs for two would come one after the other
+    const int workers = p.tile_workers > 0 && s.workers > 1 ? s.workers / CTAS_PER_SM : s.workers;
+    const dim3 grid((unsigned)workers, (unsigned)s.groups), block((unsigned)((s.heads_per_cta * s.phases + 1) * 32));
     return with_rows_kernel<T>(s.lpr, p.head_width == s.lpr * 16, [&](auto kernel) {
         return mb_launch(kernel, grid, block, rows_smem((size_t)p.lanes, s), stream, p);
     });
 }
 
+// Two of these CTAs must not share an SM, one of them and one of k_lane_rows must: at least what
+// leaves no room for two.
+constexpr size_t TILE_ALONE = 115u * 1000u;
+
 template <typename T, int SLABS>
 size_t tile_smem(size_t lanes, size_t prefixes) {
-    return TileShape<T, SLABS>::SMEM + 16u * prefixes + 6u * lanes + 16u;
+    const size_t need = TileShape<T, SLABS>::SMEM + 16u * prefixes + 6u * lanes + 16u;
+    return need > TILE_ALONE ? need : TILE_ALONE;
 }
 template <typename T, int SLABS>
 int launch_tiles(const LaneP &p, cudaStream_t stream) {
@@ -710,9 +754,12 @@ int launch_all(const LaneP &p, const Shape &s, int sm_count, cudaStream_t stream
     if (rc != 0) return rc;
     int columns = 1;
     while (columns * 4 < p.head_width) columns *= 2;
-    const size_t ctas = (size_t)p.lanes * (size_t)p.heads;
-    const dim3 grid((unsigned)p.lanes, (unsigned)p.heads), block(ctas <= 2u * (size_t)sm_count ? 512u : 128u);
-    rc = mb_launch(k_lane_merge<T>, grid, block, 0, stream, p, columns);
+    // sixteen warps for a head while the device has room for them all
+    const unsigned lanes = (unsigned)p.lanes, heads = (unsigned)p.heads;
+    if ((size_t)lanes * heads <= 2u * (size_t)sm_count)
+        rc = mb_launch(k_lane_merge<T, 16>, dim3(lanes, heads), dim3(512), 0, stream, p, columns);
+    else
+        rc = mb_launch(k_lane_merge<T, 1>, dim3(lanes, (heads + MERGE_HEADS - 1) / MERGE_HEADS), dim3(MERGE_HEADS * 32), 0, stream, p, columns);
     if (rc == 0 && launched != nullptr) *launched += p.tile_workers > 0 ? 3u : 2u;
     return rc;
 }
