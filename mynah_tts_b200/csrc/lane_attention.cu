@@ -28,6 +28,7 @@ struct LaneP {
     float scale_log2;              // scale * log2(e): scores are powers of two
     const float *qkv;
     size_t qkv_stride;
+    int qkv_vectors;               // rows of qkv start on 16 bytes
     char *k, *v;
     unsigned slots, capacity;
     size_t row_stride, slot_stride;               // elements
@@ -234,6 +235,11 @@ __device__ __forceinline__ void copy_row(unsigned to, const char *from, unsigned
 }
 __device__ __forceinline__ void bar_arrive(void *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(bar)) : "memory");
+}
+
+// `bytes` (16 or 0) bytes, the rest of 16 zeros, by the calling thread.
+__device__ __forceinline__ void copy_async(unsigned to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
 // FULL: the head fills all columns, LPR * 16.
@@ -677,7 +683,7 @@ Shape lane_shape(size_t heads, size_t head_width, size_t size, int sm_count) {
 constexpr size_t TILE_LANES = 16;
 
 int tile_workers(size_t lanes, size_t prefixes, int sm_count) {
-    return prefixes > 0 && lanes >= TILE_LANES ? sm_count : 0;      // one CTA per SM beside one of k_lane_rows
+    return prefixes > 0 && lanes >= TILE_LANES ? TILE_CTAS_PER_SM * sm_count : 0;
 }
 
 // Places of the workspace, in floats.
@@ -720,26 +726,25 @@ size_t rows_smem(size_t lanes, const Shape &s) {
 }
 template <typename T>
 int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
-    // beside k_lane_prefix an SM has room for one CTA; runs for two would come one after the other
-    const int workers = p.tile_workers > 0 && s.workers > 1 ? s.workers / CTAS_PER_SM : s.workers;
+    // Beside k_lane_prefix an SM has room for one CTA.  While that kernel is the longer one, runs for
+    // one CTA per SM are better (256 lanes of up to 500 rows behind 4,096: 68 us against 75); behind
+    // short prefixes its CTAs are soon gone and the SM takes two (64 lanes of up to 512 behind 217: 35
+    // against 38).
+    const bool beside = p.tile_workers > 0 && p.prefix_capacity > p.capacity;
+    const int workers = beside && s.workers > 1 ? s.workers / CTAS_PER_SM : s.workers;
     const dim3 grid((unsigned)workers, (unsigned)s.groups), block((unsigned)((s.heads_per_cta * s.phases + 1) * 32));
     return with_rows_kernel<T>(s.lpr, p.head_width == s.lpr * 16, [&](auto kernel) {
         return mb_launch(kernel, grid, block, rows_smem((size_t)p.lanes, s), stream, p);
     });
 }
 
-// Two of these CTAs must not share an SM, one of them and one of k_lane_rows must: at least what
-// leaves no room for two.
-constexpr size_t TILE_ALONE = 115u * 1000u;
-
 template <typename T, int SLABS>
 size_t tile_smem(size_t lanes, size_t prefixes) {
-    const size_t need = TileShape<T, SLABS>::SMEM + 16u * prefixes + 6u * lanes + 16u;
-    return need > TILE_ALONE ? need : TILE_ALONE;
+    return TileShape<T, SLABS>::SMEM + 16u * prefixes + 6u * lanes + 16u;
 }
 template <typename T, int SLABS>
 int launch_tiles(const LaneP &p, cudaStream_t stream) {
-    return mb_launch(k_lane_prefix<T, SLABS>, dim3((unsigned)p.tile_workers), dim3(TILE_THREADS), tile_smem<T, SLABS>((size_t)p.lanes, p.prefixes),
+    return mb_launch(k_lane_prefix<T, SLABS>, dim3((unsigned)p.tile_workers), dim3(TILE), tile_smem<T, SLABS>((size_t)p.lanes, p.prefixes),
                      stream, p);
 }
 
@@ -800,6 +805,7 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
     p.qkv = a->qkv;
     p.qkv_stride = a->qkv_stride;
+    p.qkv_vectors = ((uintptr_t)a->qkv & 15u) == 0 && a->qkv_stride % 4u == 0 && a->head_width % 4u == 0;
     p.k = (char *)a->cache.k;
     p.v = (char *)a->cache.v;
     p.slots = (unsigned)a->cache.slots;

@@ -11,11 +11,12 @@
 // (the others are below 2^-24 of the result).
 //
 // The blocks of all (tile, head) pairs, counted on, are cut into equal runs, one per CTA; a run
-// that ends inside a pair leaves a partial result, which k_lane_merge joins.  Two threads own a
-// row of the tile, half of a block's scores and half of the columns each; its maximum, sum and
-// weighted sum stay in registers, so tensor memory is never rescaled.  The loops over scores and
-// pieces are kept rolled: most CTAs run through them a few times only, and unrolled code was
-// fetched at 200 cycles per score.
+// that ends inside a pair leaves a partial result, which k_lane_merge joins.  A thread owns a
+// row of the tile: its maximum, sum and weighted sum stay in registers, so tensor memory is never
+// rescaled.  A block is a chain of copies, products and a softmax by four warps, so an SM takes
+// two CTAs (and one of k_lane_rows, which the memory keeps busy meanwhile) rather than wider
+// ones.  The loops over scores are kept rolled: most CTAs run through them a few times only, and
+// unrolled code was fetched at 200 cycles per score.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -24,20 +25,19 @@
 
 namespace {
 
-constexpr int TILE = 128;          // rows of a tile
-constexpr int TILE_THREADS = 256;
-constexpr unsigned TILE_TMEM = 256, TILE_P = 128;   // columns: S, then O in its place, below; p from there on
+constexpr int TILE = 128;          // rows of a tile, threads of a CTA
 constexpr int TILE_CTAS_PER_SM = 2;
 
 template <typename T, int SLABS>
 struct TileShape {
     static constexpr bool F16 = sizeof(T) == 2;
-    static constexpr int KEYS = F16 && SLABS == 1 ? 128 : 64;  // prefix rows of a block
+    static constexpr int KEYS = F16 ? 64 : 32;                 // prefix rows of a block
     static constexpr int QP = F16 ? 2 : 3, KP = F16 ? 1 : 3;   // planes of q and p, of K and V
     static constexpr int Q_SLAB = TILE * 128, K_SLAB = KEYS * 128;     // bytes of 64 columns
     static constexpr int Q_PLANE = SLABS * Q_SLAB, K_PLANE = SLABS * K_SLAB;
-    static constexpr int PIECES = KEYS * SLABS * 8 / TILE_THREADS;     // 8 elements of K and of V per thread
-    static constexpr int LOADS = F16 ? 1 : 2;                          // 16-byte loads of a piece
+    static constexpr int PIECES = KEYS * SLABS * 8 / TILE;     // 8 elements of K and of V per thread
+    // columns of tensor memory: S, then O in its place, below; p from P on
+    static constexpr unsigned P = SLABS * 64, TMEM = P + QP * KEYS / 2 <= 128 ? 128 : 256;
     static constexpr size_t SMEM = (size_t)QP * Q_PLANE + 2u * KP * K_PLANE + 1024u;
 };
 
@@ -178,30 +178,29 @@ __device__ void tile_schedule(const LaneP &p, unsigned short *voice, unsigned *r
 }
 
 template <typename T, int SLABS>
-__global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 1) k_lane_prefix(LaneP p) {
+__global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP p) {
     using C = TileShape<T, SLABS>;
     constexpr bool F16 = C::F16;
-    constexpr int KEYS = C::KEYS, QP = C::QP, KP = C::KP, PIECES = C::PIECES, LOADS = C::LOADS;
-    constexpr int HALF = KEYS / 2, COLS = SLABS * 32;      // scores and columns of a thread
+    constexpr int KEYS = C::KEYS, QP = C::QP, KP = C::KP, PER_ROW = SLABS * 8;
     extern __shared__ unsigned char sm_tile[];
     __shared__ __align__(8) unsigned long long s_bar;
     __shared__ uint32_t s_tmem;
     __shared__ unsigned s_units, s_run;
     __shared__ unsigned short s_row[TILE];                 // lanes of the tile
-    __shared__ float s_unscale[TILE], s_half[2][TILE];
+    __shared__ float s_unscale[TILE];
     unsigned char *base = sm_tile + ((1024u - (saddr(sm_tile) & 1023u)) & 1023u);
     unsigned char *sq = base, *sk = sq + QP * C::Q_PLANE, *sv = sk + KP * C::K_PLANE;
     unsigned char *rest = base + (C::SMEM - 1024u);        // schedule
     uint4 *s_prefix = reinterpret_cast<uint4 *>(rest);
     unsigned *s_rank = reinterpret_cast<unsigned *>(s_prefix + p.prefixes);
     unsigned short *s_voice = reinterpret_cast<unsigned short *>(s_rank + p.lanes);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = tid % TILE, half = tid / TILE;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     mb_pdl_wait();
     mb_pdl_trigger();
     tile_schedule<KEYS>(p, s_voice, s_rank, s_prefix, &s_units, &s_run);
     if (blockIdx.x == 0) {
-        for (int b = tid; b < p.lanes; b += TILE_THREADS) p.tile_lane[b] = s_rank[b];
-        for (int g = tid; g < (int)p.prefixes; g += TILE_THREADS) p.tile_prefix[g] = s_prefix[g];
+        for (int b = tid; b < p.lanes; b += TILE) p.tile_lane[b] = s_rank[b];
+        for (int g = tid; g < (int)p.prefixes; g += TILE) p.tile_prefix[g] = s_prefix[g];
         if (tid == 0) *p.tile_run = s_run;
     }
     const unsigned units = s_units, run = s_run;
@@ -213,13 +212,13 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&s_tmem)), "r"(TILE_TMEM) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&s_tmem)), "r"(C::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = s_tmem, my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16);    // a warp reaches 32 rows
+    const uint32_t tmem = s_tmem, my_tmem = tmem + ((uint32_t)(warp * 32) << 16);
     const int hw = p.head_width, ksteps = (hw + 15) / 16, ncols = ksteps * 16;
     const uint32_t format = F16 ? 0u : (1u << 7 | 1u << 10);
     const uint32_t idesc_s = instr_desc_f16(TILE, KEYS) | format;
@@ -239,49 +238,53 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
         const unsigned keys = min(p.prefix_length[g], p.prefix_capacity);
         unit += stop - block;
 
-        // K and V rows of a block on their way, zero beyond the prefix and beyond the head (rows
-        // that are not seen may hold anything)
+        // f16 rows of a block on their way, zero beyond the prefix and beyond the head (rows that are
+        // not seen may hold anything)
         const size_t origin = (size_t)g * p.prefix_stride + (size_t)head * hw;
         const T *pk = reinterpret_cast<const T *>(p.prefix_k) + origin, *pv = reinterpret_cast<const T *>(p.prefix_v) + origin;
-        uint4 kx[PIECES][LOADS], vx[PIECES][LOADS];
-        auto fetch = [&](unsigned block) {
+        auto bring = [&](const T *from, unsigned char *to, unsigned block) {
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int at = tid + i * TILE_THREADS, r = at / (SLABS * 8), d = at % (SLABS * 8) * 8;
+            for (int i = 0; i < C::PIECES; ++i) {
+                const int at = tid + i * TILE, r = at / PER_ROW, c = at % PER_ROW;
                 const unsigned j = block * KEYS + r;
-#pragma unroll
-                for (int l = 0; l < LOADS; ++l) {
-                    kx[i][l] = vx[i][l] = make_uint4(0, 0, 0, 0);
-                    if (j < keys && d + 4 * l < hw) {
-                        const size_t from = (size_t)j * p.prefix_row_stride + d + 4 * l;
-                        kx[i][l] = __ldg(reinterpret_cast<const uint4 *>(pk + from));
-                        vx[i][l] = __ldg(reinterpret_cast<const uint4 *>(pv + from));
-                    }
-                }
+                const bool in = j < keys && c * 8 < hw;
+                copy_async(saddr(to) + (c >> 3) * C::K_SLAB + swizzled(r, c & 7),
+                           in ? from + (size_t)j * p.prefix_row_stride + c * 8 : from, in ? 16 : 0);
             }
         };
-        fetch(block);
-        __syncthreads();                                   // s_row
-        for (int b = tid; b < p.lanes; b += TILE_THREADS)
+        __syncthreads();                                   // s_row and the queries are read no more
+        if (F16) {
+            bring(pk, sk, block);
+            bring(pv, sv, block);
+        }
+        for (int b = tid; b < p.lanes; b += TILE)
             if (s_voice[b] == g && s_rank[b] / TILE == tile) s_row[s_rank[b] % TILE] = (unsigned short)b;
         __syncthreads();
 
         // the queries: scaled, cut into planes, rows of 128 bytes per slab
-        constexpr int PER_ROW = SLABS * 8, QUERIES = 4;
+        constexpr int QUERIES = 4;
 #pragma unroll 1
-        for (int i0 = tid; i0 - lane < rows * PER_ROW; i0 += QUERIES * TILE_THREADS) {
+        for (int i0 = tid; i0 - lane < rows * PER_ROW; i0 += QUERIES * TILE) {
             float x[QUERIES][8];
 #pragma unroll
             for (int u = 0; u < QUERIES; ++u) {
-                const int i = i0 + u * TILE_THREADS, r = i / PER_ROW, c = i % PER_ROW;
+                const int i = i0 + u * TILE, r = i / PER_ROW, c = i % PER_ROW;
                 const float *q = p.qkv + (size_t)(r < rows ? s_row[r] : 0) * p.qkv_stride + head * hw + c * 8;
+                if (p.qkv_vectors && r < rows && c * 8 + 8 <= hw) {
+                    const float4 a = *reinterpret_cast<const float4 *>(q), b = *reinterpret_cast<const float4 *>(q + 4);
+                    x[u][0] = a.x; x[u][1] = a.y; x[u][2] = a.z; x[u][3] = a.w;
+                    x[u][4] = b.x; x[u][5] = b.y; x[u][6] = b.z; x[u][7] = b.w;
+                } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[u][j] = r < rows && c * 8 + j < hw ? q[j] * p.scale_log2 : 0.0f;
+                    for (int j = 0; j < 8; ++j) x[u][j] = r < rows && c * 8 + j < hw ? q[j] : 0.0f;
+                }
             }
 #pragma unroll
             for (int u = 0; u < QUERIES; ++u) {
-                const int i = i0 + u * TILE_THREADS, r = i / PER_ROW, c = i % PER_ROW;
+                const int i = i0 + u * TILE, r = i / PER_ROW, c = i % PER_ROW;
                 float most = 0.0f, up = 1.0f, down = 1.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[u][j] *= p.scale_log2;
                 if (F16) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[u][j]));
@@ -306,39 +309,49 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
                 }
             }
         }
-        const bool mine = row < rows;
-        const bool work = (warp & 3) * 32 < rows;          // a warp without a row has nothing to weigh
+        const bool mine = tid < rows;
+        const bool work = warp * 32 < rows;                // a warp without a row has nothing to weigh
         unsigned seen_head = 0, seen_from = 0;             // rows of the prefix it sees: below, and from there on
         if (mine) {
-            const LaneView w = lane_view(p, s_row[row]);
+            const LaneView w = lane_view(p, s_row[tid]);
             seen_head = w.prefix_head;
             seen_from = w.prefix_head + w.prefix_jump;
         }
-        float unscale = 1.0f, top = -INFINITY, sum = 0.0f, o[COLS];
+        float unscale = 1.0f, top = -INFINITY, sum = 0.0f, o[SLABS * 64];
 #pragma unroll
-        for (int i = 0; i < COLS; ++i) o[i] = 0.0f;
+        for (int i = 0; i < SLABS * 64; ++i) o[i] = 0.0f;
 
+#pragma unroll 1
         for (bool begun = false; block < stop; ++block, begun = true) {
             const unsigned first = block * KEYS;
+            if (F16) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            } else {
+#pragma unroll 1
+                for (int m = 0; m < 2; ++m) {              // K, then V
+                    const T *from = m ? pv : pk;
+                    uint4 x[C::PIECES][2];
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int at = tid + i * TILE_THREADS, r = at / (SLABS * 8), c = at % (SLABS * 8);
-                const unsigned to = (c >> 3) * C::K_SLAB + swizzled(r, c & 7);
-                if (F16) {
-                    *reinterpret_cast<uint4 *>(sk + to) = kx[i][0];
-                    *reinterpret_cast<uint4 *>(sv + to) = vx[i][0];
-                } else {
+                    for (int i = 0; i < C::PIECES; ++i) {
+                        const int at = tid + i * TILE, r = at / PER_ROW, d = at % PER_ROW * 8;
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const uint4 a = m ? vx[i][0] : kx[i][0], b = m ? vx[i][LOADS - 1] : kx[i][LOADS - 1];
+                        for (int l = 0; l < 2; ++l) {
+                            x[i][l] = make_uint4(0, 0, 0, 0);
+                            if (first + r < keys && d + 4 * l < hw)
+                                x[i][l] = __ldg(reinterpret_cast<const uint4 *>(from + (size_t)(first + r) * p.prefix_row_stride + d + 4 * l));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < C::PIECES; ++i) {
+                        const int at = tid + i * TILE, r = at / PER_ROW, c = at % PER_ROW;
                         uint32_t plane[4][KP];
-                        split_pair<F16>(__uint_as_float(a.x), __uint_as_float(a.y), plane[0]);
-                        split_pair<F16>(__uint_as_float(a.z), __uint_as_float(a.w), plane[1]);
-                        split_pair<F16>(__uint_as_float(b.x), __uint_as_float(b.y), plane[2]);
-                        split_pair<F16>(__uint_as_float(b.z), __uint_as_float(b.w), plane[3]);
+                        split_pair<F16>(__uint_as_float(x[i][0].x), __uint_as_float(x[i][0].y), plane[0]);
+                        split_pair<F16>(__uint_as_float(x[i][0].z), __uint_as_float(x[i][0].w), plane[1]);
+                        split_pair<F16>(__uint_as_float(x[i][1].x), __uint_as_float(x[i][1].y), plane[2]);
+                        split_pair<F16>(__uint_as_float(x[i][1].z), __uint_as_float(x[i][1].w), plane[3]);
 #pragma unroll
                         for (int j = 0; j < KP; ++j)
-                            *reinterpret_cast<uint4 *>((m ? sv : sk) + j * C::K_PLANE + to) =
+                            *reinterpret_cast<uint4 *>((m ? sv : sk) + j * C::K_PLANE + (c >> 3) * C::K_SLAB + swizzled(r, c & 7)) =
                                 make_uint4(plane[0][j], plane[1][j], plane[2][j], plane[3][j]);
                     }
                 }
@@ -364,46 +377,42 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
                 }
                 mma_commit(&s_bar);
             }
-            if (block + 1 < stop) fetch(block + 1);
-            if (!begun) unscale = mine ? s_unscale[row] : 1.0f;
+            if (!begun) unscale = mine ? s_unscale[tid] : 1.0f;
             bool done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
             parity ^= 1u;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (F16 && done && block + 1 < stop) bring(pk, sk, block + 1);
             // masked: beyond the prefix, or between the first rows and the window
             const bool all = first + KEYS <= keys && (first + KEYS <= seen_head || first >= seen_from);
-            uint32_t x[32];
-            auto scores = [&](int i) {
-                tmem_ld32u(my_tmem + half * HALF + i * 32, x);
-                tmem_ld_wait(x);
-                if (!__all_sync(MB_FULL, all)) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const unsigned j = first + half * HALF + i * 32 + k;
-                        if (!(j < keys && (j < seen_head || j >= seen_from))) x[k] = 0xff800000u;
-                    }
-                }
-            };
-            float m = -INFINITY;
+            float keep = 1.0f;
             if (done && work) {
+                uint32_t x[32];
+                auto scores = [&](int i) {
+                    tmem_ld32u(my_tmem + i * 32, x);
+                    tmem_ld_wait(x);
+                    if (!__all_sync(MB_FULL, all)) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const unsigned j = first + i * 32 + k;
+                            if (!(j < keys && (j < seen_head || j >= seen_from))) x[k] = 0xff800000u;
+                        }
+                    }
+                };
+                float m = -INFINITY;
 #pragma unroll 1
-                for (int i = 0; i < HALF / 32; ++i) {
+                for (int i = 0; i < KEYS / 32; ++i) {
                     scores(i);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) m = fmaxf(m, __uint_as_float(x[k]));
                 }
-                s_half[half][row] = m;
-            }
-            __syncthreads();
-            float keep = 1.0f;
-            if (done && work) {
-                m = fmaxf(top, fmaxf(m, s_half[half ^ 1][row]) * unscale);
+                m = fmaxf(top, m * unscale);
                 const float ref = m == -INFINITY ? 0.0f : m;
                 keep = pow2(top - ref);
                 top = m;
                 sum *= keep;
 #pragma unroll 1
-                for (int i = 0; i < HALF / 32; ++i) {
-                    if (HALF > 32) scores(i);              // one group: still there
+                for (int i = 0; i < KEYS / 32; ++i) {
+                    if (KEYS > 32) scores(i);              // one group: still there
                     uint32_t out[QP][16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
@@ -416,7 +425,7 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
                         for (int l = 0; l < QP; ++l) out[l][k] = plane[l];
                     }
 #pragma unroll
-                    for (int l = 0; l < QP; ++l) tmem_st16u(my_tmem + TILE_P + l * HALF + half * (HALF / 2) + i * 16, out[l]);
+                    for (int l = 0; l < QP; ++l) tmem_st16u(my_tmem + C::P + l * (KEYS / 2) + i * 16, out[l]);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
@@ -433,7 +442,7 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
 #pragma unroll
                         for (int b = 0; b < KP; ++b) {
                             if (!F16 && a + b > 2) continue;
-                            mma_f16_ts(tmem, tmem + TILE_P + a * HALF + s * 8, dv + (b * C::K_PLANE + s * 2048) / 16, idesc_o,
+                            mma_f16_ts(tmem, tmem + C::P + a * (KEYS / 2) + s * 8, dv + (b * C::K_PLANE + s * 2048) / 16, idesc_o,
                                        s + a + b > 0);
                         }
                 mma_commit(&s_bar);
@@ -441,11 +450,13 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
             done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
             parity ^= 1u;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (F16 && done && block + 1 < stop) bring(pv, sv, block + 1);
             if (done && work) {
 #pragma unroll
-                for (int i = 0; i < SLABS; ++i) {
-                    if (half * COLS + i * 32 >= ncols) break;
-                    tmem_ld32u(my_tmem + half * COLS + i * 32, x);
+                for (int i = 0; i < SLABS * 2; ++i) {
+                    if (i * 32 >= ncols) break;
+                    uint32_t x[32];
+                    tmem_ld32u(my_tmem + i * 32, x);
                     tmem_ld_wait(x);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[i * 32 + j] = fmaf(o[i * 32 + j], keep, __uint_as_float(x[j]));
@@ -455,27 +466,25 @@ __global__ void __launch_bounds__(TILE_THREADS, SLABS == 1 ? TILE_CTAS_PER_SM : 
             fine = __syncthreads_and(done);                // before S and the operands are written again
             if (!fine) break;
         }
-        if (fine) {
-            if (half == 1) s_half[0][row] = sum;
-            __syncthreads();
-            if (mine) {
-                const size_t at = of.y + (size_t)tile * TILE * p.heads + (size_t)head * rows + (size_t)blockIdx.x * TILE + row;
-                if (half == 0) p.tile_stat[at] = make_float2(top, sum + s_half[0][row]);
+        if (fine && mine) {
+            const size_t at = of.y + (size_t)tile * TILE * p.heads + (size_t)head * rows + (size_t)blockIdx.x * TILE + tid;
+            p.tile_stat[at] = make_float2(top, sum);
 #pragma unroll
-                for (int i = 0; i < COLS; i += 4)
-                    if (half * COLS + i < hw)
-                        *reinterpret_cast<float4 *>(p.tile_acc + at * hw + half * COLS + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-            }
+            for (int i = 0; i < SLABS * 64; i += 4)
+                if (i < hw) *reinterpret_cast<float4 *>(p.tile_acc + at * hw + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
     }
-    if (!fine && tid == 0) {
-        atomicOr(p.status, 16);
-        bar_wait(&s_bar, parity ^ 1u, TC_SPIN >> 4);       // what may still be in flight, one more bounded chance
+    if (!fine) {
+        if (tid == 0) {
+            atomicOr(p.status, 16);
+            bar_wait(&s_bar, parity ^ 1u, TC_SPIN >> 4);   // what may still be in flight, one more bounded chance
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 0)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TILE_TMEM) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
 }
 
 }  // namespace
