@@ -37,17 +37,16 @@ namespace cg = cooperative_groups;
 
 constexpr int SEL_CLUSTER = 8;     // portable cluster size
 constexpr int SEL_SHARE = 4;       // parts of one CTA, at most
-constexpr int SEL_THREADS = 1024, SEL_FIT_THREADS = 256;
+constexpr int SEL_THREADS = 512, SEL_FIT_THREADS = 256;
 constexpr int SEL_HELD = 4;        // 16-byte pieces a thread takes in a turn, and holds of a short part (FIT)
 constexpr int SEL_CAP = 512;       // tokens listed of a part
 constexpr int SEL_PAD = MB_BEAM_MAX + 1;         // lists that lanes walk side by side: no common bank
 constexpr int SEL_LIST = MB_BEAM_MAX * SEL_PAD;
 
-// A long part goes through a ring in shared memory in which a thread fills and reads only its
-// own places, so the copies need no barrier: SEL_DEPTH turns of SEL_HELD pieces are under way,
-// 192 KB of an SM's one CTA.  (Two smaller CTAs per SM lost: the CTAs of a cluster are placed
-// in pairs on half as many SMs.)
-constexpr int SEL_DEPTH = 3;
+// Long parts go through a ring in shared memory in which a thread fills and reads only its own
+// places, so the copies need no barrier: SEL_DEPTH turns of SEL_HELD pieces are under way, across
+// the parts of a CTA, 64 KB per CTA and two CTAs per SM.
+constexpr int SEL_DEPTH = 2;
 constexpr unsigned SEL_RING_BYTES = SEL_DEPTH * SEL_HELD * SEL_THREADS * sizeof(float4);
 
 struct SelPart {                   // what one part of a row found
@@ -188,14 +187,6 @@ __device__ __forceinline__ void copy_async(float4 *to, const float4 *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
-// Asks for the whole pieces of a range to be brought into L2, 64 KB at a time.
-__device__ __forceinline__ void prefetch_row(const SelRange &r) {
-    for (int v = r.whole_from; v < r.whole_to; v += 4096) {
-        const unsigned bytes = 16u * (unsigned)min(4096, r.whole_to - v);
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(r.base + v), "r"(bytes) : "memory");
-    }
-}
-
 // Maximum and sum of exponentials of the tokens a thread has seen; NaN is passed over by the
 // maximum and shows in the sum.  `most` receives the pieces' maxima.
 template <int N>
@@ -213,15 +204,21 @@ __device__ __forceinline__ void sel_take(const float4 (&x)[N], float (&most)[N],
         sum += (sel_exp(x[u].x, ref) + sel_exp(x[u].y, ref)) + (sel_exp(x[u].z, ref) + sel_exp(x[u].w, ref));
 }
 
-// The keys of a piece's tokens that reach the bound into the list; `most`: the piece's maximum.
-__device__ __forceinline__ void sel_reach(SelScratch &w, const float4 &x, float most, unsigned token, float bound) {
-    if (!(most >= bound)) return;      // nearly every piece
-    const float e[4] = {x.x, x.y, x.z, x.w};
+// The keys of the tokens that reach the bound into the list: `most` are the pieces' maxima, piece
+// u begins with token[u].
+template <int N>
+__device__ __forceinline__ void sel_reach(SelScratch &w, const float4 (&x)[N], const float (&most)[N], const unsigned (&token)[N],
+                                          float bound) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (!(e[j] >= bound) || e[j] == -INFINITY) continue;
-        const unsigned at = atomicAdd(&w.n_reach, 1u);
-        if (at < SEL_CAP) w.reach[at] = sel_key(e[j], token + j);
+    for (int u = 0; u < N; ++u) {
+        if (!(most[u] >= bound)) continue;                 // nearly every piece
+        const float e[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!(e[j] >= bound) || e[j] == -INFINITY) continue;
+            const unsigned at = atomicAdd(&w.n_reach, 1u);
+            if (at < SEL_CAP) w.reach[at] = sel_key(e[j], token[u] + j);
+        }
     }
 }
 
@@ -250,7 +247,7 @@ __device__ __forceinline__ float sel_bound(SelScratch &w, float top, int beams) 
 
 // FIT: parts of at most SEL_HELD pieces per thread.
 template <bool FIT>
-__global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 : 1) k_beam_select(SelP p) {
+__global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 : 2) k_beam_select(SelP p) {
     __shared__ SelSmem sm;
     extern __shared__ float4 ring[];
     constexpr int NT = FIT ? SEL_FIT_THREADS : SEL_THREADS, WARPS = NT / 32;
@@ -281,12 +278,51 @@ __global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 :
     auto has = [&](int i) { return i < beams * parts && !(done >> (i / parts) & 1u); };
     auto has_eos = [&](int i) { return allow && tid == 0 && (i + 1) % parts == 0; };
 
+    // what the ring is asked for next: turn f_turn of part f_part
+    constexpr int TURN = SEL_HELD * NT;
+    int f_part = rank, f_left = 0, f_place = 0;            // f_left: pieces of the part not yet asked for
+    const float4 *f_from = nullptr;
+    auto feed = [&]() {                                    // at the first part from f_part on that has pieces
+        for (f_left = 0; f_part < beams * parts; f_part += size) {
+            if (!has(f_part)) continue;
+            const SelRange r = range(f_part);
+            f_left = r.whole_to - r.whole_from;
+            f_from = r.base + r.whole_from + tid;
+            if (f_left > 0) return;
+        }
+    };
+    auto ask = [&]() {
+        if (f_left > 0) {
+            float4 *to = ring + f_place * TURN + tid;
+            if (f_left >= TURN) {
+#pragma unroll
+                for (int u = 0; u < SEL_HELD; ++u) copy_async(to + u * NT, f_from + u * NT);
+            } else {
+#pragma unroll
+                for (int u = 0; u < SEL_HELD; ++u)
+                    if (tid + u * NT < f_left) copy_async(to + u * NT, f_from + u * NT);
+            }
+            f_from += TURN;
+            f_left -= TURN;
+            if (f_left <= 0) {
+                f_part += size;
+                feed();
+            }
+        }
+        f_place = f_place + 1 == SEL_DEPTH ? 0 : f_place + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (!FIT) {
+        feed();
+#pragma unroll 1
+        for (int i = 0; i < SEL_DEPTH; ++i) ask();
+    }
+
     // this CTA's parts: rank, rank + size, ... of the request's
     for (int i = rank, q = 0; i < beams * parts; i += size, ++q) {
         if (!has(i)) continue;
         SelScratch &w = sm.work[q];
         const SelRange r = range(i);
-        if (!FIT && tid == 0 && has(i + size)) prefetch_row(range(i + size));
         // what lies beside the whole pieces: a ragged first or last one, which falls to one thread,
         // and the token behind the range
         const int edge = tid == 0 && r.whole_from > 0 ? 0 : tid == NT - 1 && r.whole_to < r.vecs ? r.vecs - 1 : -1;
@@ -307,45 +343,30 @@ __global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 :
             sel_take(x, most, top, sum);
             sel_take(beside, beside_most, top, sum);
             bound = sel_bound<NT>(w, top, beams);
-#pragma unroll
-            for (int u = 0; u < SEL_HELD; ++u) sel_reach(w, x[u], most[u], token + 4 * u * NT, bound);
+            const unsigned tokens[SEL_HELD] = {token, token + 4 * NT, token + 8 * NT, token + 12 * NT};
+            sel_reach(w, x, most, tokens, bound);
         } else {
-            constexpr int TURN = SEL_HELD * NT;
-            const int turns = whole / TURN, rest = whole - turns * TURN;   // whole turns, pieces of the last one
-            const float4 *from = at;                                       // next piece to ask for
-            float4 *to = ring + tid;
-            auto ask = [&](int turn) {
-                if (turn < turns) {
-#pragma unroll
-                    for (int u = 0; u < SEL_HELD; ++u) copy_async(to + u * NT, from + u * NT);
-                } else if (turn == turns) {
-#pragma unroll
-                    for (int u = 0; u < SEL_HELD; ++u)
-                        if (tid + u * NT < rest) copy_async(to + u * NT, from + u * NT);
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                from += TURN;
-                to = to == ring + (SEL_DEPTH - 1) * TURN + tid ? ring + tid : to + TURN;
-            };
-            for (int turn = 0; turn < SEL_DEPTH; ++turn) ask(turn);
             sel_take(beside, beside_most, top, sum);
-            for (int turn = 0; turn <= turns; ++turn, token += 4 * TURN) {
+            bound = INFINITY;
+            for (int turn = 0, left = whole; left > 0; ++turn, left -= TURN, token += 4 * TURN) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(SEL_DEPTH - 1) : "memory");
+                const float4 *place = ring + f_place * TURN + tid;         // the one that is asked for next
 #pragma unroll
-                for (int u = 0; u < SEL_HELD; ++u) x[u] = to[u * NT];      // the place asked for next
-                if (turn == turns)
+                for (int u = 0; u < SEL_HELD; ++u) x[u] = place[u * NT];
+                if (left < TURN)
 #pragma unroll
                     for (int u = 0; u < SEL_HELD; ++u)
-                        if (tid + u * NT >= rest) x[u] = no_tokens();
-                ask(turn + SEL_DEPTH);
+                        if (tid + u * NT >= left) x[u] = no_tokens();
+                ask();
                 sel_take(x, most, top, sum);
                 if ((turn & (turn + 1)) == 0) bound = sel_bound<NT>(w, top, beams);
-#pragma unroll
-                for (int u = 0; u < SEL_HELD; ++u) sel_reach(w, x[u], most[u], token + 4 * u * NT, bound);
+                const unsigned tokens[SEL_HELD] = {token, token + 4 * NT, token + 8 * NT, token + 12 * NT};
+                sel_reach(w, x, most, tokens, bound);
             }
+            if (whole <= 0) bound = sel_bound<NT>(w, top, beams);
         }
-        sel_reach(w, beside[0], beside_most[0], (unsigned)(r.origin + 4 * edge), bound);
-        sel_reach(w, beside[1], beside_most[1], (unsigned)p.eos, bound);
+        const unsigned beside_tokens[2] = {(unsigned)(r.origin + 4 * edge), (unsigned)p.eos};
+        sel_reach(w, beside, beside_most, beside_tokens, bound);
         if (sum != sum) {              // NaN among the logits, or +inf: the sum again without them
             sum = 0.0f;
             top = -INFINITY;
@@ -645,8 +666,7 @@ extern "C" int mb_beam_select(const mb_beam_select_args *a, mb_stream stream) {
         return sel_launch(k_beam_select<true>, p, a->requests, size, SEL_FIT_THREADS, 0u, (cudaStream_t)stream, nullptr);
     }
     // long parts: the cluster size with the fewest parts one after the other, counting the waves
-    // that the device needs for all clusters (24 requests of 16 beams: 6 CTAs, all at once, and
-    // three parts each; 8 CTAs take two waves of two)
+    // that the device needs for all clusters
     int best = 0, least = 0;
     for (int size = SEL_CLUSTER; size >= 1; --size) {
         const int share = (pieces + size - 1) / size;
