@@ -679,11 +679,25 @@ Shape lane_shape(size_t heads, size_t head_width, size_t size, int sm_count) {
     return s;
 }
 
-// From TILE_LANES lanes the prefixes go through the tensor cores.
-constexpr size_t TILE_LANES = 16;
+// Whether the prefixes go through the tensor cores, from what the host knows: every lane's prefix
+// full, the lanes spread over the prefixes.  Walked like own rows they come from L2, at 14 (f32) and
+// 10 (f16) bytes a picosecond and some; a tile costs a launch, its queries and partials, 5 us, and 5
+// or 4 us for every block that its CTA takes one after the other.  With 12 heads of 64 and own rows
+// of 100 .. 300, tiles against walking: 24 lanes behind 4,000 f32 rows 47 / 54 us, 16 lanes 44 / 41;
+// 48 lanes behind 1,000 34 / 35, 32 lanes 30 / 27; 48 behind 217 26 / 20; f16: 16 behind 4,000 27 / 34,
+// 12 lanes 24 / 26; 32 behind 1,000 20 / 23, 16 lanes 20 / 19.
+constexpr size_t TILE_LANES = 8;   // fewer lanes never use them (and have no workspace for them)
 
-int tile_workers(size_t lanes, size_t prefixes, int sm_count) {
-    return prefixes > 0 && lanes >= TILE_LANES ? TILE_CTAS_PER_SM * sm_count : 0;
+bool use_tiles(size_t lanes, size_t heads, size_t head_width, size_t size, size_t prefixes, size_t prefix_capacity, size_t window,
+               size_t sinks, int sm_count) {
+    if (prefixes == 0 || lanes < TILE_LANES) return false;
+    const bool f16 = size == 2u;
+    const size_t seen = window > 0 && window + sinks < prefix_capacity ? window + sinks : prefix_capacity;
+    const size_t full = (lanes + TILE - 1) / TILE, tiles = prefixes > full ? (prefixes < lanes ? prefixes : lanes) : full;
+    const size_t keys = f16 ? TileShape<__half, 1>::KEYS : TileShape<float, 1>::KEYS, at_once = (size_t)(TILE_CTAS_PER_SM * sm_count);
+    const size_t blocks = tiles * heads * ((prefix_capacity + keys - 1) / keys), turns = (blocks + at_once - 1) / at_once;
+    const double walk_us = 2.0 * (double)(lanes * seen) * (double)(heads * head_width * size) / (f16 ? 10e6 : 14e6);
+    return walk_us > 5.0 + (f16 ? 4.0 : 5.0) * (double)turns;
 }
 
 // Places of the workspace, in floats.
@@ -692,7 +706,7 @@ struct Places { size_t offset, stat, acc, tile_lane, tile_prefix, tile_run, tile
 Places lane_places(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count) {
     const Shape s = lane_shape(heads, head_width, 4u, sm_count);      // workers go by the heads alone
     const size_t parts = (size_t)s.workers + lanes;
-    const size_t workers = (size_t)tile_workers(lanes, prefixes, sm_count);
+    const size_t workers = prefixes > 0 && lanes >= TILE_LANES ? (size_t)(TILE_CTAS_PER_SM * sm_count) : 0u;
     const size_t rows = workers > 0 ? lanes * heads + workers * TILE : 0u;
     Places w;
     size_t at = 0;
@@ -836,7 +850,9 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     p.step = s.step;
     p.row_bytes = s.row_bytes;
     p.row_pitch = s.row_pitch;
-    p.tile_workers = tile_workers(a->lanes, a->prefixes, a->sm_count);
+    if (use_tiles(a->lanes, a->heads, a->head_width, a->cache.type == MB_F16 ? 2u : 4u, a->prefixes, a->prefix_capacity, a->window,
+                  a->sinks, a->sm_count))
+        p.tile_workers = TILE_CTAS_PER_SM * a->sm_count;
     p.tile_lane = reinterpret_cast<unsigned *>(a->workspace + w.tile_lane);
     p.tile_prefix = reinterpret_cast<uint4 *>(a->workspace + w.tile_prefix);
     p.tile_run = reinterpret_cast<unsigned *>(a->workspace + w.tile_run);

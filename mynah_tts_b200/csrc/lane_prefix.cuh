@@ -33,6 +33,7 @@ struct TileShape {
     static constexpr bool F16 = sizeof(T) == 2;
     static constexpr int KEYS = F16 ? 64 : 32;                 // prefix rows of a block
     static constexpr int QP = F16 ? 2 : 3, KP = F16 ? 1 : 3;   // planes of q and p, of K and V
+    static constexpr int ORDERS = F16 ? 1 : 2;                 // products of planes a and b with a + b up to this
     static constexpr int Q_SLAB = TILE * 128, K_SLAB = KEYS * 128;     // bytes of 64 columns
     static constexpr int Q_PLANE = SLABS * Q_SLAB, K_PLANE = SLABS * K_SLAB;
     static constexpr int PIECES = KEYS * SLABS * 8 / TILE;     // 8 elements of K and of V per thread
@@ -362,19 +363,23 @@ __global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP 
             if (tid == 0) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t dq = smem_desc_sw128(saddr(sq)), dk = smem_desc_sw128(saddr(sk));
+                uint32_t more = 0u;
+                // the smallest products first: what they add to is not yet rounded to the size of the result
 #pragma unroll
-                for (int s = 0; s < SLABS * 4; ++s) {
-                    if (s >= ksteps) break;
-                    const unsigned off = (unsigned)(s & 3) * 2u;           // 16 columns, in 16-byte units
+                for (int order = C::ORDERS; order >= 0; --order)
 #pragma unroll
-                    for (int a = 0; a < QP; ++a)
+                    for (int a = 0; a < QP; ++a) {
+                        const int b = order - a;
+                        if (b < 0 || b >= KP) continue;
 #pragma unroll
-                        for (int b = 0; b < KP; ++b) {
-                            if (!F16 && a + b > 2) continue;
+                        for (int s = 0; s < SLABS * 4; ++s) {
+                            if (s >= ksteps) break;
+                            const unsigned off = (unsigned)(s & 3) * 2u;   // 16 columns, in 16-byte units
                             mma_f16(tmem, dq + (a * C::Q_PLANE + (s >> 2) * C::Q_SLAB) / 16 + off,
-                                    dk + (b * C::K_PLANE + (s >> 2) * C::K_SLAB) / 16 + off, idesc_s, s + a + b > 0);
+                                    dk + (b * C::K_PLANE + (s >> 2) * C::K_SLAB) / 16 + off, idesc_s, more);
+                            more = 1u;
                         }
-                }
+                    }
                 mma_commit(&s_bar);
             }
             if (!begun) unscale = mine ? s_unscale[tid] : 1.0f;
@@ -435,16 +440,19 @@ __global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP 
             if (tid == 0) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t dv = smem_desc_sw128_mn(saddr(sv), C::K_SLAB);
+                uint32_t more = 0u;
 #pragma unroll
-                for (int s = 0; s < KEYS / 16; ++s)
+                for (int order = C::ORDERS; order >= 0; --order)
 #pragma unroll
-                    for (int a = 0; a < QP; ++a)
+                    for (int a = 0; a < QP; ++a) {
+                        const int b = order - a;
+                        if (b < 0 || b >= KP) continue;
 #pragma unroll
-                        for (int b = 0; b < KP; ++b) {
-                            if (!F16 && a + b > 2) continue;
-                            mma_f16_ts(tmem, tmem + C::P + a * (KEYS / 2) + s * 8, dv + (b * C::K_PLANE + s * 2048) / 16, idesc_o,
-                                       s + a + b > 0);
+                        for (int s = 0; s < KEYS / 16; ++s) {
+                            mma_f16_ts(tmem, tmem + C::P + a * (KEYS / 2) + s * 8, dv + (b * C::K_PLANE + s * 2048) / 16, idesc_o, more);
+                            more = 1u;
                         }
+                    }
                 mma_commit(&s_bar);
             }
             done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
