@@ -532,6 +532,10 @@ typedef struct {
  * and the next mynah_cuda_sync reports it.  A slot may appear once per call.  Rows of the
  * cache that a lane does not see may hold anything.
  *
+ * A prefix that enough lanes share is multiplied on the tensor cores, once for 128 lanes; the
+ * environment, read when the backend is opened, overrides the choice: MYNAH_B200_LANE_TILES=0
+ * (and MYNAH_B200_NO_TC=1) never, =1 for any 8 lanes.  Results agree to 32-bit rounding.
+ *
  * Limits: 1 .. 1024 lanes, 1 .. 64 heads, head_width up to 128 in multiples of 16 bytes of the
  * cache's type, lanes * (capacity + prefix_capacity) < 2^32. */
 typedef struct {

@@ -353,6 +353,10 @@ int mynah_b200_open(void **state, int device, int quant, int strict, char *error
         return -1;
     }
     st->own_stream = 1;
+    {
+        const char *no_tc = getenv("MYNAH_B200_NO_TC"), *tiles = getenv("MYNAH_B200_LANE_TILES");
+        st->lane_tiles = no_tc != NULL && strcmp(no_tc, "0") != 0 ? 0 : tiles != NULL ? strcmp(tiles, "0") != 0 : -1;
+    }
     if (st->strict) {
         const char *env = getenv("MYNAH_B200_LIBM_TABLES");
         if (env == NULL || strcmp(env, "0") != 0) libm_tables_for(st);

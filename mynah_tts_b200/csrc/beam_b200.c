@@ -130,6 +130,7 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
     m.workspace = a->dev_workspace;
     m.status = st->d_status;
     m.sm_count = st->sm_count;
+    m.tiles = st->lane_tiles;
     m.launched = &launched;
     device_scope scope;
     if (enter_device(st, &scope, error, cap) != 0) return -1;

@@ -850,8 +850,11 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     p.step = s.step;
     p.row_bytes = s.row_bytes;
     p.row_pitch = s.row_pitch;
-    if (use_tiles(a->lanes, a->heads, a->head_width, a->cache.type == MB_F16 ? 2u : 4u, a->prefixes, a->prefix_capacity, a->window,
-                  a->sinks, a->sm_count))
+    bool tiles = a->tiles > 0 && a->prefixes > 0 && a->lanes >= TILE_LANES;
+    if (a->tiles < 0)
+        tiles = use_tiles(a->lanes, a->heads, a->head_width, a->cache.type == MB_F16 ? 2u : 4u, a->prefixes, a->prefix_capacity,
+                          a->window, a->sinks, a->sm_count);
+    if (tiles)
         p.tile_workers = TILE_CTAS_PER_SM * a->sm_count;
     p.tile_lane = reinterpret_cast<unsigned *>(a->workspace + w.tile_lane);
     p.tile_prefix = reinterpret_cast<uint4 *>(a->workspace + w.tile_prefix);

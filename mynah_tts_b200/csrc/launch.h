@@ -422,6 +422,7 @@ typedef struct {
     float *workspace;           /* mb_lane_attention_floats() */
     int *status;
     int sm_count;
+    int tiles;                  /* prefixes on the tensor cores: 0 never, 1 wherever possible, -1 where faster */
     unsigned *launched;         /* incremented by the number of kernels the call enqueued */
 } mb_lane_attn_args;
 size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count);

@@ -25,6 +25,17 @@ def be():
     b.close()
 
 
+@pytest.fixture(scope="module")
+def tiled():
+    """A backend that multiplies every shared prefix on the tensor cores."""
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("MYNAH_B200_LANE_TILES", "1")
+        b = Backend("f32")
+    b.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield b
+    b.close()
+
+
 def dev(a):
     return torch.from_numpy(np.ascontiguousarray(a)).cuda()
 
@@ -115,9 +126,9 @@ class Lanes:
             s = self.slots[b]
             want, spread = ref.lane(q, k, v, want_store["k"][s, :self.capacity, :width], want_store["v"][s, :self.capacity, :width],
                                     self.lengths[b], pk, pv, self.heads, self.scale, self.window, self.sinks)
-            off = np.abs(out[b, :width] - want)
-            assert (np.isfinite(out[b, :width]) == np.isfinite(want)).all(), (b, self.lengths[b], P)
             fine = np.isfinite(want)
+            assert np.array_equal(out[b, :width][~fine], want[~fine], equal_nan=True), (b, self.lengths[b], P)
+            off = np.abs(out[b, :width] - np.where(fine, want, 0))
             assert (off[fine] <= spread[fine]).all(), (b, self.lengths[b], P, float((off / spread)[fine].max()))
             assert (out[b, width:] == 7.0).all()
         for m in "kv":
@@ -126,9 +137,13 @@ class Lanes:
             self.store[m] = want_store[m]
 
 
-def attend(be, *a, **kw):
+def attend(be, *a, tiles=None, **kw):
+    """tiles: whether the prefixes have to go through the tensor cores, a launch of their own."""
     x = Lanes(be, *a, **kw)
+    before = be.launch_count
     x.bind()()
+    if tiles is not None:
+        assert be.launch_count - before == (3 if tiles else 2)
     be.sync()
     x.check()
     return x
@@ -162,6 +177,77 @@ def test_one_prefix_for_all(be, kind, lanes, prefix):
 @pytest.mark.parametrize("hw", [16, 48, 128])
 def test_prefix_with_other_head_widths(be, kind, hw):
     attend(be, kind, 3, hw, [b % 5 for b in range(70)], 6, prefix_lengths=[143], seed=hw)
+
+
+# the prefixes as tiles: lanes around the 128 rows of one, rows around its blocks of 32 (f32) and 64
+# (f16), heads that leave columns of a slab empty and heads of two slabs
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("lanes, prefix, heads, hw", [(8, 1, 3, 64), (31, 4096, 3, 64), (128, 64, 12, 64), (129, 65, 2, 64), (200, 31, 2, 64),
+                                                      (97, 2017, 1, 128), (140, 250, 3, 48), (300, 100, 2, 24), (257, 301, 1, 16),
+                                                      (130, 500, 1, 72), (64, 1399, 5, 104), (1024, 33, 1, 32)])
+def test_prefix_tiles(tiled, kind, lanes, prefix, heads, hw):
+    r = np.random.default_rng(lanes + hw)
+    attend(tiled, kind, heads, hw, [int(n) for n in r.integers(0, 9, lanes)], 9, prefix_lengths=[prefix], seed=lanes + prefix,
+           prefix_spare=3, tiles=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_tiles_of_several_prefixes(tiled, kind):
+    """Two of them with more than one tile, one empty, one of a single row, lanes without any."""
+    r = np.random.default_rng(8)
+    lengths = [600, 0, 1, 190, 63]
+    voices = [int(v) for v in r.choice([0, 0, 0, 0, 1, 2, 3, 3, 3, 4, 5], 480)]          # 5: no such prefix
+    attend(tiled, kind, 2, 64, [int(n) for n in r.integers(0, 5, 480)], 6, prefix_lengths=lengths, voices=voices, seed=2, tiles=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("window, sinks", [(250, 4), (190, 130), (30, 195), (1, 200), (7, 0)])
+def test_tiles_behind_a_window(tiled, kind, window, sinks):
+    r = np.random.default_rng(window)
+    attend(tiled, kind, 2, 64, [0, 1, 5, 90, 210, 260, 900] + [int(n) for n in r.integers(0, 300, 143)], window + sinks + 1,
+           prefix_lengths=[200], window=window, sinks=sinks, seed=window, tiles=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_tiles_with_strides_and_odd_values(tiled, kind):
+    """Padded rows, unaligned queries, spare slots; then rows of extreme sizes, infinite and NaN
+    rows of one prefix, and a live count."""
+    r = np.random.default_rng(3)
+    attend(tiled, kind, 2, 64, [b % 4 for b in range(150)], 5, prefix_lengths=[190], pad=8, gap=3, qkv_gap=5, spare=4, prefix_spare=2,
+           seed=4, tiles=True)
+    for spread in (30.0, 1e-4):
+        attend(tiled, kind, 2, 64, [b % 4 for b in range(150)], 5, prefix_lengths=[190], spread=spread, seed=5, tiles=True)
+    x = Lanes(tiled, kind, 2, 64, [3] * 300, 4, prefix_lengths=[150, 170], voices=[int(v) for v in r.integers(0, 2, 300)], seed=6)
+    # a row that one head of every lane looks away from, far larger than the others
+    x.prefix["k"][:, 77] = 0.0
+    x.prefix["v"][:, 77, 5] = 30000.0
+    x.qkv[:, 0] = 30.0
+    x.prefix["k"][:, 77, 0] = -30.0
+    # and, in the second prefix, values that are no numbers, which its lanes see
+    x.prefix["v"][1, 3, 70] = np.inf
+    x.prefix["v"][1, 9, 71] = -np.inf
+    x.prefix["k"][1, 169, 64] = -np.inf if kind == "f16" else np.nan
+    x.dp, x.d_qkv = {m: dev(x.prefix[m]) for m in "kv"}, dev(x.qkv)
+    x.live = ints([299])
+    x.bind()()
+    tiled.sync()
+    x.check(live=299)
+
+
+def test_the_choice_of_tiles(be, tiled):
+    """Long prefixes of many lanes are worth a launch, short ones are walked."""
+    r = np.random.default_rng(1)
+    attend(be, "f16", 12, 64, [int(n) for n in r.integers(0, 4, 64)], 4, prefix_lengths=[3000], seed=1, tiles=True)
+    attend(be, "f32", 12, 64, [int(n) for n in r.integers(0, 4, 64)], 4, prefix_lengths=[217], seed=2, tiles=False)
+    attend(tiled, "f32", 2, 64, [1] * 7, 4, prefix_lengths=[40], seed=3, tiles=False)
+    attend(tiled, "f32", 2, 64, [1] * 8, 4, prefix_lengths=[40], seed=4, tiles=True)
+    attend(tiled, "f32", 2, 64, [1] * 80, 4, seed=5, tiles=False)
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("MYNAH_B200_NO_TC", "1")
+        simt = Backend("f32")
+    simt.set_stream(torch.cuda.current_stream().cuda_stream)
+    attend(simt, "f16", 12, 64, [1] * 64, 4, prefix_lengths=[3000], seed=1, tiles=False)
+    simt.close()
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
@@ -289,12 +375,13 @@ def test_offsets_beyond_32_bits(be):
     assert np.array_equal(k[0, :n + 1].cpu().numpy(), host["k"]) and np.array_equal(v[0, :n + 1].cpu().numpy(), host["v"])
 
 
-def test_captured_calls_follow_lengths_and_run_beside_each_other(be):
+def test_captured_calls_follow_lengths_and_run_beside_each_other(be, monkeypatch):
     """Two graphs with workspaces of their own replayed on two streams at once, lengths moved on
     between replays; a step by step run of the same lanes agrees bit for bit."""
     runs = []
-    for seed in (20, 21):
-        lanes = Lanes(be, "f32", 4, 32, [3, 0, 11, 6] * 10, 40, prefix_lengths=[50], seed=seed)
+    for seed, kind, tiles in ((20, "f32", "0"), (21, "f16", "1")):
+        lanes = Lanes(be, kind, 4, 32, [3, 0, 11, 6] * 25, 40, prefix_lengths=[300], seed=seed)
+        monkeypatch.setenv("MYNAH_B200_LANE_TILES", tiles)
         other = Backend("f32")
         stream = torch.cuda.Stream()
         other.set_stream(stream.cuda_stream)
@@ -312,8 +399,8 @@ def test_captured_calls_follow_lengths_and_run_beside_each_other(be):
         for lanes, other, stream, graph in runs:
             lanes.check()
             first = lanes.d_out.clone()
-            lanes.bind()()
-            be.sync()
+            lanes.bind(other)()
+            other.sync()
             assert torch.equal(first, lanes.d_out)
             lanes.lengths = [n + 1 for n in lanes.lengths]
             lanes.d_len += 1
