@@ -537,7 +537,7 @@ typedef struct {
  * (and MYNAH_B200_NO_TC=1) never, =1 for any 8 lanes.  Results agree to 32-bit rounding.
  *
  * Limits: 1 .. 1024 lanes, 1 .. 64 heads, head_width up to 128 in multiples of 16 bytes of the
- * cache's type, lanes * (capacity + prefix_capacity) < 2^32. */
+ * cache's type, lanes * (capacity + prefix_capacity) <= 2^30. */
 typedef struct {
     size_t lanes, heads, head_width;   /* cache.width = heads * head_width */
     float scale;
@@ -574,7 +574,7 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
  * gets score -inf, token 0 and its own index as parent.  A finished beam that is picked, and
  * a beam whose token is eos_id, is done.  dev_score_out may be dev_score and dev_done_out
  * dev_done; the other arrays are distinct.
- * Limits: 1 .. 16 beams, vocab < 2^30, logits 4-byte aligned. */
+ * Limits: 1 .. 16 beams, 1 .. 2^24 requests, vocab < 2^30, logits 4-byte aligned. */
 typedef struct {
     const float *dev_logits;           /* [requests * beams] rows */
     size_t requests, beams, vocab, logits_stride;
@@ -591,8 +591,10 @@ int mynah_b200_beam_select(void *state, const mynah_b200_beam_select_args *args,
 
 /* Own rows 0 .. min(dev_length[parent], capacity) - 1 of every beam become its parent's, in
  * place, for K and V of all layers (a cache used as a ring moves whole); rows behind them
- * stay.  A parent that is not a beam of the request, or a slot that is not below `slots`,
- * moves nothing.  dev_length_out receives every lane's new length; it is an array of its own.
+ * stay.  A slot may appear once per call.  A parent that is not a beam of the request, and a
+ * slot (the lane's or its parent's) that is not below `slots`, moves nothing.  dev_length_out
+ * receives every lane's new length, its own where nothing could be moved; it is an array of its
+ * own.
  * Limits: 1 .. 16 beams, requests and 2 * layers up to 65535. */
 typedef struct {
     mynah_b200_lane_cache cache;

@@ -560,7 +560,8 @@ __global__ void __launch_bounds__(256) k_beam_reorder(ReorderP p) {
         const unsigned from_length = __shfl_sync(MB_FULL, length, parent & 31);
         const size_t from = __shfl_sync(MB_FULL, (unsigned long long)slot, parent & 31);
         const unsigned rows = from_length < p.capacity ? from_length : (unsigned)p.capacity;
-        const bool moves = mine && parent != (unsigned)lane && rows > 0 && slot < p.slots && from < p.slots && slot != from;
+        const bool there = slot < p.slots && from < p.slots;
+        const bool moves = mine && parent != (unsigned)lane && rows > 0 && there && slot != from;
         const unsigned mask = __ballot_sync(MB_FULL, moves);
         if (moves) {
             const int i = __popc(mask & ((1u << lane) - 1u));
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(256) k_beam_reorder(ReorderP p) {
             s_rows[i] = rows;
         }
         if (lane == 0) s_moved = __popc(mask);
-        if (mine && p.length_out != nullptr && plane == 0 && blockIdx.x == 0) p.length_out[at] = from_length;
+        if (mine && p.length_out != nullptr && plane == 0 && blockIdx.x == 0) p.length_out[at] = there ? from_length : length;
     }
     __syncthreads();
     const int moved = s_moved;

@@ -27,6 +27,10 @@ static int refuse(const char *message, char *error, size_t cap) {
     return -1;
 }
 
+/* What the kernels count in 32 bits: rows of all lanes, and two blocks of them for each of 64 heads. */
+#define MB_LANE_ROWS_MAX ((size_t)1 << 30)
+
+static int aligned4(const void *p) { return ((uintptr_t)p & 3u) == 0; }
 static int aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 /* 0 when rows of `width` elements can be walked in 16-byte pieces. */
@@ -64,7 +68,7 @@ size_t mynah_b200_lane_attention_workspace(const void *state, size_t lanes, size
                                            size_t prefixes, size_t prefix_capacity) {
     const mb_state *st = (const mb_state *)state;
     if (st == NULL || !attention_sizes_ok(lanes, heads, head_width) || prefixes > MB_LANES_MAX ||
-        prefix_capacity > 0xffffffffu / lanes)
+        prefix_capacity > MB_LANE_ROWS_MAX / lanes)
         return 0;
     return mb_lane_attention_floats(lanes, heads, head_width, prefixes, st->sm_count);
 }
@@ -79,7 +83,7 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
     if (a->cache.width != width || a->head_width % per != 0)
         return refuse("cache width must be heads * head_width, head_width a multiple of 16 bytes", error, cap);
     if (a->dev_qkv == NULL || a->qkv_stride < 3u * width || a->dev_length == NULL || a->dev_out == NULL ||
-        a->out_stride < width)
+        a->out_stride < width || !aligned4(a->dev_qkv) || !aligned4(a->dev_out))
         return refuse("invalid lane attention buffers", error, cap);
     if (a->dev_slot == NULL && a->cache.slots < a->lanes)
         return refuse("fewer slots than lanes", error, cap);
@@ -93,8 +97,8 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
             (a->prefixes > 1 && a->prefix_stride == 0) || !aligned16(a->dev_prefix_k) || !aligned16(a->dev_prefix_v))
             return refuse("prefix rows must be 16-byte aligned and prefix_row_stride at least the width", error, cap);
     }
-    if (a->lanes * (a->cache.capacity + prefix_capacity) > 0xffffffffu)
-        return refuse("lanes * (capacity + prefix_capacity) must be below 2^32", error, cap);
+    if (a->lanes * (a->cache.capacity + prefix_capacity) > MB_LANE_ROWS_MAX)
+        return refuse("lanes * (capacity + prefix_capacity) must be at most 2^30", error, cap);
     if (a->window > 0 && (a->window > a->cache.capacity || a->sinks > a->cache.capacity - a->window))
         return refuse("a windowed cache must hold window + sinks rows", error, cap);
     if (a->dev_workspace == NULL || !aligned16(a->dev_workspace) ||
@@ -146,8 +150,8 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
 int mynah_b200_beam_select(void *state, const mynah_b200_beam_select_args *a, char *error, size_t cap) {
     mb_state *st = (mb_state *)state;
     if (st == NULL || a == NULL) return refuse("invalid beam selection request", error, cap);
-    if (a->requests == 0 || a->requests > 0x0fffffffu || a->beams == 0 || a->beams > MB_BEAM_MAX)
-        return refuse("beam selection takes 1..16 beams and at least one request", error, cap);
+    if (a->requests == 0 || a->requests > (size_t)1 << 24 || a->beams == 0 || a->beams > MB_BEAM_MAX)
+        return refuse("beam selection takes 1..16 beams and 1..2^24 requests", error, cap);
     if (a->vocab == 0 || a->vocab >= (size_t)1 << 30 || a->codebook_size > a->vocab || a->logits_stride < a->vocab)
         return refuse("beam selection vocabulary out of range", error, cap);
     if (a->dev_logits == NULL || a->dev_score == NULL || a->dev_score_out == NULL || a->dev_token == NULL ||

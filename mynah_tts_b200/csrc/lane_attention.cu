@@ -206,7 +206,7 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
     }
     if (tid == 0) {
         off[p.lanes] = carry;
-        const unsigned each = (carry + workers - 1) / workers;
+        const unsigned each = (carry + workers - 1) / workers;        // carry <= 2^30
         *run = max((each + step - 1) / step * step, 2u * step);
     }
     __syncthreads();

@@ -5,10 +5,13 @@
 //     S = Q K^T,   p = 2^(S - max),   O += p V
 // with both products by tcgen05.mma, S, p and O in tensor memory.  The prefix is read once per
 // 128 lanes, which is the point; without it every lane would stream it.  Operands are 16-bit,
-// results are to be 32-bit: an f16 cache is exact as it is, and a query (first scaled by a power
-// of two into [1, 2)) and a weight are two f16 planes, 22 bits; an f32 cache, query and weight
-// are three bf16 planes, 24 bits and the exponent range of f32, and six of the nine products
-// (the others are below 2^-24 of the result).
+// results are to be 32-bit: an f16 cache is exact as it is, and a query and a weight are two f16
+// planes, 22 bits.  Both planes end at f16's smallest value, 2^-24, so both are scaled to the top of
+// its range: a query by a power of two that puts its largest element into [2^14, 2^15), a weight by
+// 2^15 (what is kept as the maximum is 15 less).  Then what is lost is below 2^-38 of the largest
+// element or weight, also where thousands of rows of small weight outweigh a few.  An f32 cache,
+// query and weight are three bf16 planes, 24 bits and the exponent range of f32, and six of the nine
+// products (the others are below 2^-24 of the result).
 //
 // The blocks of all (tile, head) pairs, counted on, are cut into equal runs, one per CTA; a run
 // that ends inside a pair leaves a partial result, which k_lane_merge joins.  A thread owns a
@@ -33,6 +36,7 @@ struct TileShape {
     static constexpr bool F16 = sizeof(T) == 2;
     static constexpr int KEYS = F16 ? 64 : 32;                 // prefix rows of a block
     static constexpr int QP = F16 ? 2 : 3, KP = F16 ? 1 : 3;   // planes of q and p, of K and V
+    static constexpr float WEIGHT_TOP = F16 ? 15.0f : 0.0f;    // the largest weight, a power of two
     static constexpr int ORDERS = F16 ? 1 : 2;                 // products of planes a and b with a + b up to this
     static constexpr int Q_SLAB = TILE * 128, K_SLAB = KEYS * 128;     // bytes of 64 columns
     static constexpr int Q_PLANE = SLABS * Q_SLAB, K_PLANE = SLABS * K_SLAB;
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP 
         __syncthreads();
 
         // the queries: scaled, cut into planes, rows of 128 bytes per slab
-        constexpr int QUERIES = 4;
+        constexpr int QUERIES = 4, QUERY_TOP = 14;
 #pragma unroll 1
         for (int i0 = tid; i0 - lane < rows * PER_ROW; i0 += QUERIES * TILE) {
             float x[QUERIES][8];
@@ -291,11 +295,12 @@ __global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP 
                     for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[u][j]));
 #pragma unroll
                     for (int o = PER_ROW / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(MB_FULL, most, o));
-                    // 2^e <= most < 2^(e + 1); zero and what is not finite stay as they are
+                    // 2^e <= most < 2^(e + 1); what is not finite stays as it is, and so does what is
+                    // so small that all its scores are 0
                     const int e = (int)(__float_as_uint(most) >> 23) - 127;
-                    if (e > -126 && e < 127) {
-                        up = __uint_as_float((unsigned)(127 - e) << 23);
-                        down = __uint_as_float((unsigned)(127 + e) << 23);
+                    if (e > -100 && e < 127) {
+                        up = __uint_as_float((unsigned)(127 + QUERY_TOP - e) << 23);
+                        down = __uint_as_float((unsigned)(127 - QUERY_TOP + e) << 23);
                     }
                 }
                 if (r < rows) {
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP 
 #pragma unroll
                     for (int k = 0; k < 32; ++k) m = fmaxf(m, __uint_as_float(x[k]));
                 }
-                m = fmaxf(top, m * unscale);
+                m = fmaxf(top, fmaf(m, unscale, -C::WEIGHT_TOP));
                 const float ref = m == -INFINITY ? 0.0f : m;
                 keep = pow2(top - ref);
                 top = m;

@@ -51,7 +51,8 @@ def attention(cache=None, **change):
     (dict(prefix_capacity=0), {}, "prefixes"), (dict(prefixes=1025), {}, "prefixes"),
     (dict(prefix_row_stride=124), {}, "prefix rows"), (dict(dev_prefix_v=A + 4), {}, "prefix rows"),
     (dict(prefixes=2, prefix_stride=0), {}, "prefix rows"), (dict(prefix_stride=2050), {}, "prefix rows"),
-    (dict(prefix_capacity=1 << 30), {}, "2^32"), ({}, dict(capacity=(1 << 31) - 1), "2^32"),
+    (dict(prefix_capacity=1 << 30), {}, "2^30"), ({}, dict(capacity=(1 << 31) - 1), "2^30"),
+    (dict(prefix_capacity=(1 << 28) - 31), {}, "2^30"), (dict(dev_qkv=A + 2), {}, "buffers"), (dict(dev_out=A + 1), {}, "buffers"),
     (dict(window=33), {}, "window"), (dict(window=30, sinks=3), {}, "window"),
     (dict(window=1, sinks=(1 << 64) - 1), {}, "window"),
     (dict(dev_workspace=None), {}, "workspace"), (dict(dev_workspace=A + 4), {}, "workspace"),
@@ -84,7 +85,7 @@ def select(**change):
 
 
 @pytest.mark.parametrize("change", [
-    dict(requests=0), dict(beams=0), dict(beams=17), dict(vocab=0), dict(vocab=1 << 30, logits_stride=1 << 30),
+    dict(requests=0), dict(beams=0), dict(requests=(1 << 24) + 1), dict(beams=17), dict(vocab=0), dict(vocab=1 << 30, logits_stride=1 << 30),
     dict(codebook_size=65), dict(logits_stride=63), dict(dev_logits=None), dict(dev_score=None), dict(dev_score_out=None),
     dict(dev_token=None), dict(dev_parent=None), dict(dev_parent=A), dict(dev_logits=A + 2)])
 def test_beam_select_refuses(change):

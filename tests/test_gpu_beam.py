@@ -234,6 +234,43 @@ def test_tiles_with_strides_and_odd_values(tiled, kind):
     x.check(live=299)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_tiles_keep_small_weights(tiled, kind):
+    """2,000 rows of weight 2.5e-8 beside one of weight 1 whose value is 0.  All terms of the result
+    are positive, so it is off by the roundings of its terms relative to ITSELF (the largest value
+    is at most three times the mean, which `bound` already counts)."""
+    r = np.random.default_rng(11)
+    x = Lanes(tiled, kind, 2, 64, [0] * 40, 2, prefix_lengths=[2001], seed=11)
+    x.qkv[:] = 0.0
+    x.qkv[:, [0, 64]], x.qkv[:, [128, 192]], x.qkv[:, 256:] = 14.0, -10.0, r.uniform(0.5, 1.5, (40, 128))
+    x.prefix["k"][:] = 0.0
+    x.prefix["k"][:, 1:, [0, 64]] = -10.0
+    x.prefix["v"][:] = r.uniform(0.5, 1.5, x.prefix["v"].shape)
+    x.prefix["v"][:, 0] = 0.0
+    x.dp, x.d_qkv = {m: dev(x.prefix[m]) for m in "kv"}, dev(x.qkv)
+    x.bind()()
+    tiled.sync()
+    got = x.d_out.cpu().numpy()
+    for b in range(0, 40, 13):
+        q, k, v = (x.qkv[b, i * 128:(i + 1) * 128] for i in range(3))
+        want, _ = ref.lane(q, k, v, *(np.zeros((2, 128), NP[kind]) for _ in "kv"), 0, x.prefix["k"][0], x.prefix["v"][0], 2, 0.125, 0, 0)
+        tolerance = 3 * ref.bound(np.float64(17.5), 64, 2002) * want
+        assert (np.abs(got[b] - want) <= tolerance).all()
+    x.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_tiles_keep_small_elements_of_a_query(tiled, kind):
+    """One element of a million that every row multiplies by zero."""
+    x = Lanes(tiled, kind, 2, 64, [0] * 40, 2, prefix_lengths=[300], seed=12)
+    x.qkv[:, [5, 69]], x.qkv[:, [133, 197]] = 1e6, 0.0
+    x.prefix["k"][..., [5, 69]] = 0.0
+    x.dp, x.d_qkv = {m: dev(x.prefix[m]) for m in "kv"}, dev(x.qkv)
+    x.bind()()
+    tiled.sync()
+    x.check()
+
+
 def test_the_choice_of_tiles(be, tiled):
     """Long prefixes of many lanes are worth a launch, short ones are walked."""
     r = np.random.default_rng(1)
@@ -590,6 +627,17 @@ def test_reorder_live_count_missing_slots_and_identity(be):
     want = k.copy()
     want[1, :, :4] = k[0, :, :4]
     assert np.array_equal(dk.cpu().numpy(), want) and out.cpu().tolist() == [4, 4, 4, -1, -1, -1]
+    # nothing to be had from a lane without a slot, and nowhere to put it: lengths stay
+    dk = dev(k)
+    cache = be.lane_cache("f32", dk.data_ptr(), dv.data_ptr(), 6, 10, 16)
+    cache.layer_stride = 160
+    parent, length = ints([2, 0, 0, 5, 3, 4]), ints([3, 4, 5, 6, 7, 8])
+    be.beam_reorder(cache, requests=2, beams=3, slot=slot.data_ptr(), parent=parent.data_ptr(), length=length.data_ptr(),
+                    length_out=out.data_ptr(), live=live.data_ptr())
+    be.sync()
+    want = k.copy()
+    want[1, :, :3] = k[0, :, :3]
+    assert np.array_equal(dk.cpu().numpy(), want) and out.cpu().tolist() == [3, 3, 5, -1, -1, -1]
     before = dk.clone()
     parent = ints([0, 1, 2, 0, 1, 2])
     be.beam_reorder(cache, requests=2, beams=3, parent=parent.data_ptr(), length=length.data_ptr())
