@@ -221,8 +221,11 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
 // ROWS_DEPTH steps, across the lanes of a run: up to 100 KB per CTA, two CTAs per SM.  Rows lie
 // row_pitch apart there, an odd multiple of the 16 * LPR bytes that the lanes of a row read at
 // once (any 16-byte multiple for eight lanes), so that a warp's reads share no bank.
-// (48 lanes x 1,029 f16 rows, 152 MB, with the merge: loads into registers 40 us, 16-byte copies
-// by every thread 34 us, bulk copies ROWS_US us.)
+// 48 lanes x 1,029 f16 rows of 12 heads of 64, 152 MB, with the merge: loads into registers 40 us,
+// 16-byte copies by every thread 38, bulk copies 33.1 (4.6 TB/s).  The rows take 21 us of it, at 7
+// TB/s; the others are the schedule (2), the first rows' latency (2), uneven ends (3) and the merge
+// (5).  Four steps of 8 rows instead of two of 16: 32.0, but 8 rows at a time cost 4 to 15% wherever
+// rows come from L2 or one CTA has an SM to itself.
 constexpr int ROWS_DEPTH = 2;
 constexpr size_t ROWS_STAGE = 50u * 1024u;       // bytes of a step, at most
 
@@ -353,7 +356,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const unsigned i = (phase + u * p.phases) * GROUPS + group;
-                at_u[u] = from + (size_t)(min(i, most) * p.row_pitch);         // no row: the last one, with weight 0
+                at_u[u] = from + (size_t)(min(i, most) * p.row_pitch);
                 x[u] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -378,6 +381,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
             for (int u = 0; u < U; ++u) {
                 const float e = pow2(x[u] - ref);
                 sum += e;
+                if ((phase + u * p.phases) * GROUPS + group > most) continue;  // weight 0 times an infinity would be NaN
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     if (!FULL && (j * LPR + part) * PER >= p.head_width) continue;

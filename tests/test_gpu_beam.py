@@ -355,6 +355,19 @@ def test_infinite_and_nan_rows_that_are_seen(be, kind):
     assert np.isfinite(out[:10]).all() and np.isinf(out[10:, 4]).all() and np.isnan(out[10:, 32:]).all()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("heads, hw", [(12, 64), (2, 64), (3, 128), (4, 16)])
+def test_an_infinite_value_in_the_last_row(be, kind, heads, hw):
+    """Wherever a run of rows ends, its last one counts once."""
+    x = Lanes(be, kind, heads, hw, list(range(1, 60)), 70, seed=13)
+    for b, n in enumerate(x.lengths):
+        x.store["v"][x.slots[b], n - 1, b % x.width] = np.inf
+    x.d = {m: dev(x.store[m]) for m in "kv"}
+    x.bind()()
+    be.sync()
+    x.check()
+
+
 def test_lanes_behind_the_live_count_stay(be):
     for live in (0, 1, 5, 12, 99):
         x = Lanes(be, "f32", 3, 32, [4, 0, 9, 2] * 3, 10, prefix_lengths=[20], seed=9)
