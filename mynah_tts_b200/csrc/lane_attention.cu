@@ -222,7 +222,7 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
 // row_pitch apart there, an odd multiple of the 16 * LPR bytes that the lanes of a row read at
 // once (any 16-byte multiple for eight lanes), so that a warp's reads share no bank.
 // 48 lanes x 1,029 f16 rows of 12 heads of 64, 152 MB, with the merge: loads into registers 40 us,
-// 16-byte copies by every thread 38, bulk copies 33.1 (4.6 TB/s).  The rows take 21 us of it, at 7
+// 16-byte copies by every thread 34, bulk copies 33 (4.6 TB/s).  The rows take 21 us of it, at 7
 // TB/s; the others are the schedule (2), the first rows' latency (2), uneven ends (3) and the merge
 // (5).  Four steps of 8 rows instead of two of 16: 32.0, but 8 rows at a time cost 4 to 15% wherever
 // rows come from L2 or one CTA has an SM to itself.
@@ -687,9 +687,10 @@ Shape lane_shape(size_t heads, size_t head_width, size_t size, int sm_count) {
 // full, the lanes spread over the prefixes.  Walked like own rows they come from L2, at 14 (f32) and
 // 10 (f16) bytes a picosecond and some; a tile costs a launch, its queries and partials, 5 us, and 5
 // or 4 us for every block that its CTA takes one after the other.  With 12 heads of 64 and own rows
-// of 100 .. 300, tiles against walking: 24 lanes behind 4,000 f32 rows 47 / 54 us, 16 lanes 44 / 41;
-// 48 lanes behind 1,000 34 / 35, 32 lanes 30 / 27; 48 behind 217 26 / 20; f16: 16 behind 4,000 27 / 34,
-// 12 lanes 24 / 26; 32 behind 1,000 20 / 23, 16 lanes 20 / 19.
+// of 100 .. 300, tiles / walking: f32 24 lanes behind 4,000 rows 45.9 / 53.3 us, 16 lanes 43.8 / 40.2;
+// 48 behind 1,000 31.7 / 34.3, 32 lanes 28.7 / 26.2; 48 behind 217 25.5 / 19.4; f16 16 behind 4,000
+// 25.3 / 33.7, 12 lanes 21.9 / 25.2 (the estimate still walks), 8 lanes 21.5 / 19.7; 32 behind 1,000
+// 18.5 / 22.1, 16 lanes 19.0 / 17.5; 128 behind 217 32.5 / 29.7.
 constexpr size_t TILE_LANES = 8;   // fewer lanes never use them (and have no workspace for them)
 
 bool use_tiles(size_t lanes, size_t heads, size_t head_width, size_t size, size_t prefixes, size_t prefix_capacity, size_t window,
@@ -744,11 +745,12 @@ size_t rows_smem(size_t lanes, const Shape &s) {
 }
 template <typename T>
 int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
-    // Beside k_lane_prefix an SM has room for one CTA.  While that kernel is the longer one, runs for
-    // one CTA per SM are better (256 lanes of up to 500 rows behind 4,096: 68 us against 75); behind
-    // short prefixes its CTAs are soon gone and the SM takes two (64 lanes of up to 512 behind 217: 35
-    // against 38).
-    const bool beside = p.tile_workers > 0 && p.prefix_capacity > p.capacity;
+    // Beside two f16 CTAs of k_lane_prefix an SM has room for one CTA of this: runs for one CTA per SM
+    // (32 lanes behind 1,000 rows: 18.5 us against 21.6; 16 behind 4,000: 25.3 / 27.2; where the own rows
+    // go on for as long as the tiles, 256 lanes of up to 500 behind 4,096, it is 74.6 / 73.3).  Beside
+    // two f32 ones it has none, and takes two when they have ended (48 lanes behind 1,000: 31.7 us
+    // against 33.9 with runs for one).
+    const bool beside = p.tile_workers > 0 && sizeof(T) == 2;
     const int workers = beside && s.workers > 1 ? s.workers / CTAS_PER_SM : s.workers;
     const dim3 grid((unsigned)workers, (unsigned)s.groups), block((unsigned)((s.heads_per_cta * s.phases + 1) * 32));
     return with_rows_kernel<T>(s.lpr, p.head_width == s.lpr * 16, [&](auto kernel) {
