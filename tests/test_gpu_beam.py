@@ -288,6 +288,68 @@ def test_the_choice_of_tiles(be, tiled):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("lanes, prefixes", [(300, 70), (1024, 1024)])
+def test_tiles_of_many_prefixes(tiled, kind, lanes, prefixes):
+    """More prefixes than a warp has lanes; most tiles hold a few lanes, some prefixes none."""
+    r = np.random.default_rng(prefixes)
+    lengths = [int(n) for n in r.integers(0, 40, prefixes)]
+    attend(tiled, kind, 1, 32, [b % 3 for b in range(lanes)], 4, prefix_lengths=lengths,
+           voices=[int(v) for v in r.integers(0, prefixes, lanes)], seed=lanes, tiles=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_slots_and_prefixes_by_default_and_interleaved_caches(be, tiled, kind):
+    """No slot and prefix arrays: lane b in slot b, behind prefix 0.  K and V rows side by side in
+    one buffer, the prefix rows those of another slot of it."""
+    r = np.random.default_rng(17)
+    lanes, heads, hw, capacity, prefix = 20, 2, 32, 24, 17
+    width, t = heads * hw, NP[kind]
+    both = r.normal(size=(lanes + 1, capacity, 2, width)).astype(t)          # the last slot: the prefix
+    qkv = r.normal(size=(lanes, 3 * width)).astype(np.float32)
+    lengths = [int(n) for n in r.integers(0, capacity, lanes)]
+    for b in (be, tiled):
+        d, d_qkv, d_len, d_p = dev(both), dev(qkv), ints(lengths), ints([prefix])
+        out = torch.zeros((lanes, width), device="cuda")
+        size, row = both.itemsize, 2 * width
+        at = d.data_ptr() + lanes * capacity * row * size
+        cache = b.lane_cache(kind, d.data_ptr(), d.data_ptr() + width * size, lanes, capacity, width, row_stride=row,
+                             slot_stride=capacity * row)
+        floats = b.lane_attention_workspace(lanes, heads, hw, 1, prefix)
+        space = torch.empty(floats, device="cuda")
+        b.lane_attention(cache, lanes=lanes, heads=heads, head_width=hw, scale=-0.3, qkv=d_qkv.data_ptr(), length=d_len.data_ptr(),
+                         prefixes=1, prefix_k=at, prefix_v=at + width * size, prefix_capacity=prefix, prefix_row_stride=row,
+                         prefix_length=d_p.data_ptr(), out=out.data_ptr(), workspace=space.data_ptr(), workspace_floats=floats)
+        b.sync()
+        want = both.copy()
+        for i in range(lanes):
+            q, k, v = (qkv[i, j * width:(j + 1) * width] for j in range(3))
+            o, spread = ref.lane(q, k, v, want[i, :, 0], want[i, :, 1], lengths[i], both[lanes, :prefix, 0], both[lanes, :prefix, 1],
+                                 heads, -0.3, 0, 0)
+            assert (np.abs(out[i].cpu().numpy() - o) <= spread).all()
+        assert np.array_equal(d.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("live", [0, 1])
+def test_no_lane_or_one_in_use(be, tiled, live):
+    for b in (be, tiled):
+        x = Lanes(b, "f32", 2, 32, [4] * 12, 9, prefix_lengths=[30], seed=18)
+        x.live = ints([live])
+        x.bind()()
+        b.sync()
+        x.check(live=live)
+        assert all(np.array_equal(x.d[m].cpu().numpy(), x.store[m], equal_nan=True) for m in "kv")
+
+
+def test_scale_of_zero_weighs_all_rows_alike(be, tiled):
+    for b in (be, tiled):
+        x = Lanes(b, "f16", 2, 64, [4] * 12, 9, prefix_lengths=[30], seed=19)
+        x.scale = 0.0
+        x.bind()()
+        b.sync()
+        x.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
 def test_several_prefixes_one_empty_and_lanes_without(be, kind):
     r = np.random.default_rng(8)
     voices = [int(v) for v in r.integers(0, 6, 90)]          # 5: no such prefix
@@ -530,6 +592,34 @@ def test_select(be, requests, beams, vocab):
     check_select(be, logits, score, (r.random((requests, beams)) < 0.2).astype(np.int64), codebook, vocab - 1,
                  (r.random(requests) < 0.5).astype(np.int64), stride=vocab + 3, offset=beams % 4)
     check_select(be, logits, score, None, vocab, vocab + 5, None)
+
+
+@pytest.mark.parametrize("beams", [1, 4, 16])
+def test_select_with_only_the_end_allowed(be, beams):
+    """No token but eos_id: one candidate a beam; where it is not allowed either, none."""
+    r = np.random.default_rng(beams)
+    logits, score = r.normal(size=(3, beams, 40)), r.normal(size=(3, beams))
+    check_select(be, logits.astype(np.float32), score.astype(np.float32), None, 0, 39, np.array([1, 0, 1]))
+    check_select(be, logits.astype(np.float32), score.astype(np.float32), None, 0, 40, None)
+
+
+@pytest.mark.parametrize("vocab", [4096, 4097, 8192, 8193, 16384, 16385, 32769])
+def test_select_around_the_parts_of_a_row(be, vocab):
+    """Rows that fit in registers whole or cut in two, four or eight, and the next size; the best
+    tokens on both sides of every cut."""
+    r = np.random.default_rng(vocab)
+    for beams in (1, 2, 4):
+        logits = r.normal(size=(2, beams, vocab)).astype(np.float32)
+        for cut in range(1, 8):
+            at = vocab * cut // 8
+            logits[:, :, max(0, at - 2):at + 2] += 6
+        check_select(be, logits, r.normal(size=(2, beams)).astype(np.float32), None, vocab, vocab, None)
+
+
+def test_select_many_requests(be):
+    r = np.random.default_rng(3)
+    check_select(be, r.normal(size=(5000, 2, 11)).astype(np.float32), r.normal(size=(5000, 2)).astype(np.float32), None, 9, 10,
+                 r.integers(0, 2, 5000))
 
 
 def test_select_in_place_and_first_step(be):
