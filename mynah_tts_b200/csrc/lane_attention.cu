@@ -159,17 +159,35 @@ __device__ __forceinline__ LaneView lane_rows_view(const LaneP &p, int b) {
     return w;
 }
 
-// Rows of the lanes, counted on, and the length of a run: every CTA forms them (lanes <= 1024).
-__device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int workers, int step) {
+// Rows of the lanes, counted on, and the length of a run: every CTA forms them (lanes <= 1024).  Few
+// lanes are counted in whole runs, so that no run takes from two of them, which the whole launch
+// would wait for (8 lanes of 347 rows: 9.5 us, 10.6 otherwise); `end` is where their rows end.
+constexpr int FEW_LANES = 32;
+__device__ __forceinline__ bool few_lanes(const LaneP &p, int workers) {
+    return p.lanes > 1 && p.lanes <= FEW_LANES && 8 * p.lanes <= workers;
+}
+
+__device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *end, unsigned *run, int workers, int step) {
     __shared__ unsigned warp_sum_s[32];
+    // whole steps, one at least (256 rows of one lane: 6.8 us, with two at least 7.4)
+    const auto run_of = [step](unsigned rows, unsigned among) {
+        return max(((rows + among - 1) / among + step - 1) / step * step, (unsigned)step);     // rows <= 2^30
+    };
+    const bool few = few_lanes(p, workers);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = (blockDim.x + 31) >> 5;
     unsigned carry = 0;
-    if (p.lanes <= 32) {               // one warp, one barrier
+    if (p.lanes <= FEW_LANES) {        // one warp, one barrier
         if (warp == 0) {
             unsigned n = 0;
             if (lane < p.lanes) {
                 const LaneView w = lane_rows_view(p, lane);
                 n = w.prefix_rows + w.own_rows;
+            }
+            const unsigned rows = n;
+            if (few) {
+                const unsigned each = run_of(__reduce_add_sync(MB_FULL, n), workers - p.lanes);
+                n = (n + each - 1) / each * each;
+                if (lane == 0) *run = each;
             }
             unsigned x = n;
 #pragma unroll
@@ -177,7 +195,10 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
                 const unsigned y = __shfl_up_sync(MB_FULL, x, o);
                 if (lane >= o) x += y;
             }
-            if (lane < p.lanes) off[lane] = x - n;
+            if (lane < p.lanes) {
+                off[lane] = x - n;
+                end[lane] = x - n + rows;
+            }
             carry = __shfl_sync(MB_FULL, x, 31);
         }
     } else for (int b0 = 0; b0 < p.lanes; b0 += blockDim.x) {
@@ -206,9 +227,7 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *run, int 
     }
     if (tid == 0) {
         off[p.lanes] = carry;
-        const unsigned each = (carry + workers - 1) / workers;        // carry <= 2^30
-        // whole steps, one at least (256 rows of one lane: 6.8 us, with two at least 7.4)
-        *run = max((each + step - 1) / step * step, (unsigned)step);
+        if (!few) *run = run_of(carry, workers);
     }
     __syncthreads();
 }
@@ -250,7 +269,7 @@ __device__ __forceinline__ void copy_async(unsigned to, const void *from, int by
 template <typename T, int LPR, bool FULL>
 __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
     extern __shared__ uint4 sm_rows_dyn[];
-    __shared__ unsigned s_run;
+    __shared__ unsigned s_run, s_end[FEW_LANES];
     __shared__ float s_acc[WARPS_MAX][MB_LANE_HEAD_WIDTH_MAX];
     __shared__ float2 s_stat[WARPS_MAX];
     __shared__ __align__(8) unsigned long long s_full[ROWS_DEPTH], s_empty[ROWS_DEPTH];
@@ -273,11 +292,12 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
     const auto last_wait = [&]() {
         if (p.tile_workers > 0) mb_pdl_wait();
     };
-    lane_schedule(p, sm_off, &s_run, gridDim.x, GROUPS * p.phases);
+    lane_schedule(p, sm_off, s_end, &s_run, gridDim.x, GROUPS * p.phases);
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         for (int i = threadIdx.x; i <= p.lanes; i += blockDim.x) p.offset[i] = sm_off[i];
         if (threadIdx.x == 0) p.offset[p.lanes + 1] = s_run;
     }
+    const auto end_of = [&](int b) { return p.lanes <= FEW_LANES ? s_end[b] : sm_off[b + 1]; };      // of lane b's rows
     const unsigned total = sm_off[p.lanes], run = s_run;
     const unsigned long long begin = (unsigned long long)blockIdx.x * run;
     if (begin >= total) { last_wait(); return; }
@@ -300,11 +320,11 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
         for (unsigned steps = 0; at < end && fine; ++b) {
             if (sm_off[b + 1] <= at) continue;
             unsigned r0 = at - sm_off[b];
-            const unsigned last = min(end, sm_off[b + 1]) - sm_off[b];
+            const unsigned last = min(end, end_of(b)) - sm_off[b];
             const LaneView w = lane_rows_view(p, b);
             const char *own = p.k + w.slot * p.slot_stride * sizeof(T) + column;
             const char *shared = p.prefix_k + w.prefix * p.prefix_stride * sizeof(T) + column;
-            at += last - r0;
+            at = min(end, sm_off[b + 1]);
             for (; r0 < last && fine; r0 += step) {
                 if (steps++ >= ROWS_DEPTH) fine = __all_sync(MB_FULL, bar_wait(&s_empty[stage], parity ^ 1u, TC_SPIN));
                 if (!fine) break;
@@ -334,7 +354,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
     const int head = min(wanted, p.heads - 1), group = lane / LPR, part = lane % LPR;
     const char *mine = ring + (size_t)((head - blockIdx.y * p.heads_per_cta) * p.head_width + part * PER) * sizeof(T);
     while (at < end) {
-        const unsigned first = at - sm_off[b], last = min(end, sm_off[b + 1]) - sm_off[b];
+        const unsigned first = at - sm_off[b], last = min(end, end_of(b)) - sm_off[b];
         if (last == first) { ++b; continue; }
         float q[16], acc[16], top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -451,7 +471,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
                             make_float4(acc[j * PER + i], acc[j * PER + i + 1], acc[j * PER + i + 2], acc[j * PER + i + 3]);
             }
         }
-        at += last - first;
+        at = min(end, sm_off[b + 1]);
         ++b;
     }
     last_wait();
