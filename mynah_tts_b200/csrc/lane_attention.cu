@@ -242,9 +242,9 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *end, unsi
 // row_pitch apart there, an odd multiple of the 16 * LPR bytes that the lanes of a row read at
 // once (any 16-byte multiple for eight lanes), so that a warp's reads share no bank.
 // 48 lanes x 1,029 f16 rows of 12 heads of 64, 152 MB, with the merge: loads into registers 40 us,
-// 16-byte copies by every thread 34, bulk copies 33 (4.6 TB/s).  The rows take 21 us of it, at 7
+// 16-byte copies by every thread 34, bulk copies 32.5 (4.7 TB/s).  The rows take 21 us of it, at 7
 // TB/s; the others are the schedule (2), the first rows' latency (2), uneven ends (3) and the merge
-// (5).  Four steps of 8 rows instead of two of 16: 32.0, but 8 rows at a time cost 4 to 15% wherever
+// (5).  Four steps of 8 rows instead of two of 16 save 1 us, but 8 rows at a time cost 4 to 15% wherever
 // rows come from L2 or one CTA has an SM to itself.
 constexpr int ROWS_DEPTH = 2;
 constexpr size_t ROWS_STAGE = 50u * 1024u;       // bytes of a step, at most
