@@ -10,7 +10,8 @@
 // Bound by reading every lane's K and V rows once.  The rows of all lanes, counted on, are cut
 // into equal runs, one per resident CTA (k_lane_rows), whatever the lanes' lengths: a run that
 // ends inside a lane leaves a partial result (maximum, sum, weighted sum), and k_lane_merge
-// joins a lane's partials in row order, adds the new row and appends it.
+// joins a lane's partials in row order, adds the new row and appends it.  A prefix of many lanes is
+// read once per 128 of them (lane_prefix.cuh).
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -487,7 +488,9 @@ namespace {
 // head by `warps` warps: one where there are many heads of lanes, sixteen where there are few (a
 // lane alone has hundreds of partials).  Four columns per thread; threads of the same columns take
 // every slices-th partial, MERGE_U at a time.  A lane whose cache is full or whose slot does not
-// exist is left out and sets the status word.
+// exist is left out and sets the status word.  Bound by latency, the partials come from L2: 5 us
+// behind the last rows for 48 lanes x 12 heads, of which three dependent trips to memory.  For 5
+// lanes of 3 heads and 120 partials sixteen warps take 22 us with the rows, eight 22.6, four 24.3.
 constexpr int MERGE_U = 4;
 
 struct Merged { float top, sum; float4 acc; };
