@@ -610,7 +610,7 @@ int mynah_b200_beam_reorder(void *state, const mynah_b200_beam_reorder_args *arg
 /* The same for a decoder's slots (HOST arrays): lane request * beams + beam lives in slot
  * slots[lane], each slot once; parents[lane] is the beam it continues.  Self K/V of all layers
  * and the slots' lengths follow; cross K/V stay (the beams of a request share their text).
- * Synchronous. */
+ * The decoder's width is a multiple of 4.  Synchronous. */
 int mynah_b200_decoder_reorder(void *decoder, const unsigned *slots, const unsigned *parents, size_t requests,
                                size_t beams, char *error, size_t cap);
 

@@ -1192,6 +1192,10 @@ int mynah_b200_decoder_reorder(void *decoder, const unsigned *slots, const unsig
         mb_set_error(error, cap, "reorder takes 1..16 beams per request and at most the decoder's slots");
         return -1;
     }
+    if (d->width % 4u != 0) {          /* rows are moved in 16-byte pieces */
+        mb_set_error(error, cap, "reorder takes a decoder width in multiples of 4");
+        return -1;
+    }
     const size_t n = requests * beams;
     unsigned *lanes = (unsigned *)malloc(3u * n * sizeof(unsigned));
     unsigned char *used = (unsigned char *)calloc(d->slots, 1u);

@@ -119,6 +119,15 @@ def test_decoder_reorder_refuses_without_a_decoder():
     assert b"reorder" in err.value
 
 
+def test_decoder_reorder_refuses_rows_that_are_not_16_byte_pieces():
+    """A block of ones instead of a decoder: its width is odd, its slots are plenty; nothing else
+    of it may be read before the refusal."""
+    decoder, err = C.create_string_buffer(b"\xff" * (1 << 16)), C.create_string_buffer(capi.ERR_CAP)
+    two = (C.c_uint * 2)(0, 1)
+    assert capi.lib().mynah_b200_decoder_reorder(decoder, two, two, 1, 2, err, capi.ERR_CAP) == -1
+    assert b"multiples of 4" in err.value
+
+
 def test_bound_calls_report_a_refusal():
     be = Backend.__new__(Backend)
     be.lib, be.state = capi.lib(), None
