@@ -489,8 +489,7 @@ namespace {
 // lane alone has hundreds of partials).  Four columns per thread; threads of the same columns take
 // every slices-th partial, MERGE_U at a time.  A lane whose cache is full or whose slot does not
 // exist is left out and sets the status word.  Bound by latency, the partials come from L2: 5 us
-// behind the last rows for 48 lanes x 12 heads, of which three dependent trips to memory.  For 5
-// lanes of 3 heads and 120 partials sixteen warps take 22 us with the rows, eight 22.6, four 24.3.
+// behind the last rows for 48 lanes x 12 heads, of which three dependent trips to memory.
 constexpr int MERGE_U = 4;
 
 struct Merged { float top, sum; float4 acc; };
@@ -803,7 +802,9 @@ int launch_all(const LaneP &p, const Shape &s, int sm_count, cudaStream_t stream
     if (rc != 0) return rc;
     int columns = 1;
     while (columns * 4 < p.head_width) columns *= 2;
-    // sixteen warps for a head while the device has room for them all
+    // Sixteen warps for a head while the device has room for them all: with the rows 6.9 us for one
+    // lane of 12 heads (one warp 8.6), 9.6 for 8 (10.3), 21.2 for 5 of 3 heads and 120 partials (34.9); one
+    // warp beyond: 48 lanes of 12 heads 32.5 us (sixteen 40.3), 256 lanes behind tiles 66.8 (126.6).
     const unsigned lanes = (unsigned)p.lanes, heads = (unsigned)p.heads;
     if ((size_t)lanes * heads <= 2u * (size_t)sm_count)
         rc = mb_launch(k_lane_merge<T, 16>, dim3(lanes, heads), dim3(512), 0, stream, p, columns);
