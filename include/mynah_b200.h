@@ -568,8 +568,10 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
  * picked.  With s_b the score of beam b, x_b its logits and lse_b the logarithm of the sum of
  * exp(x_b) over the tokens that may be picked, token t continues beam b with the score
  * s_b + x_bt - lse_b; a finished beam (dev_done) has one continuation, eos_id with s_b.
- * Scores are formed and compared in 64 bits and stored in 32.  Order: higher score, lower
- * beam, higher logit, lower token.  A logit that is NaN or -inf, and a continuation whose
+ * Order: higher score, lower beam, higher logit, lower token, by scores in 64 bits: log-sums
+ * are off by at most 2^-16 + vocab * 2^-38 (1e-8 as a rule), and those of beams whose continuations
+ * come closer than twice that to a pick are formed again in 64 bits; equal rows and scores are
+ * equal wherever the rows lie.  A stored score is off by its log-sum and its rounding to 32 bits.  A logit that is NaN or -inf, and a continuation whose
  * score is (a beam of score -inf is dead), is never picked; a place for which nothing is left
  * gets score -inf, token 0 and its own index as parent.  A finished beam that is picked, and
  * a beam whose token is eos_id, is done.  dev_score_out may be dev_score and dev_done_out

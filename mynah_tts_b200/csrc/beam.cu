@@ -31,22 +31,29 @@ namespace cg = cooperative_groups;
 // are listed in all.  A list that is full all the same (thousands of equal logits, or logits
 // that rise along the vocabulary) is replaced by one pass over the part per place.
 //
-// Scores are formed in 64 bits: beams differ by less than a rounding of a 32-bit sum often
-// enough to change a pick.  The sums of exponentials are 32-bit per thread (at most a few
-// hundred terms, each off by 1e-7 of itself) and 64-bit across threads.
+// The order is that of scores in 64 bits, equal ones by beam: beams differ by less than a rounding
+// of a 32-bit sum often enough to change a pick.  A 64-bit exponential per logit would bind the
+// kernel by its arithmetic, so a log-sum is formed of 32-bit terms, summed in 32 bits by a thread (see
+// SEL_FOLD) and in 64 across them, and is off by at most sel_eps; and where a continuation
+// that is picked lies within twice that of another beam's, the log-sums of those beams are formed
+// again in 64 bits, in an order that goes by the tokens alone (equal rows give equal sums wherever
+// they lie), and the picks are made again.  Beams farther apart than that cannot change places: a pair
+// that does has been a pick and a list's head.
 
 constexpr int SEL_CLUSTER = 8;     // portable cluster size
 constexpr int SEL_SHARE = 4;       // parts of one CTA, at most
 constexpr int SEL_THREADS = 512, SEL_FIT_THREADS = 256;
 constexpr int SEL_HELD = 4;        // 16-byte pieces a thread takes in a turn, and holds of a short part (FIT)
 constexpr int SEL_CAP = 512;       // tokens listed of a part
+constexpr float SEL_SLACK = 8.0f;  // what a logit may be above its thread's base
+constexpr int SEL_FOLD = 32;       // turns that a thread sums in 32 bits, or half of all
 constexpr int SEL_PAD = MB_BEAM_MAX + 1;         // lists that lanes walk side by side: no common bank
 constexpr int SEL_LIST = MB_BEAM_MAX * SEL_PAD;
 
 // Long parts go through a ring in shared memory in which a thread fills and reads only its own
 // places, so the copies need no barrier: SEL_DEPTH turns of SEL_HELD pieces are under way, across
 // the parts of a CTA, 64 KB per CTA and two CTAs per SM.  24 requests x 16 beams x 50,000, 76.8 MB:
-// loads into registers with a wait for each turn 87 us, this 29 (2.6 TB/s).  What bounds it is that
+// loads into registers with a wait for each turn 87 us, this 30 (2.6 TB/s).  What bounds it is that
 // the clusters' CTAs come in pairs on 96 of 148 SMs, each with two rows to walk one after the other
 // (64 requests reach 3.7 TB/s).
 constexpr int SEL_DEPTH = 2;
@@ -71,9 +78,20 @@ struct SelScratch {                // of one part while it is worked on
 struct SelSmem {
     SelPart part[MB_BEAM_MAX];     // first CTA: all parts of the request
     SelScratch work[SEL_SHARE];
-    double score[SEL_LIST];        // first CTA: the continuations of the request
-    unsigned long long order[SEL_LIST], key[SEL_LIST];
+    union {
+        struct {                   // first CTA, at the end: the continuations of the request
+            double score[SEL_LIST];
+            unsigned long long order[SEL_LIST], key[SEL_LIST];
+            unsigned near[SEL_LIST];       // first bits of the order of what is 2 sel_eps above the continuation
+        };
+        struct {                   // before: sums of turns, per thread, and their bases
+            double folded[SEL_THREADS];
+            float folded_base[SEL_THREADS];
+        };
+    };
     int taken[MB_BEAM_MAX];
+    unsigned close;                // not 0: a pick may have come close to another beam's continuation
+    unsigned close_beams;          // those that did
 };
 
 // Order-preserving bits of a float.
@@ -134,12 +152,15 @@ __device__ __forceinline__ float4 sel_load(const SelRange &r, int v) {
     return x;
 }
 
-// exp(x - top) for x <= top
+// exp(x - top) for x below top, or no more than SEL_SLACK above it
 __device__ __forceinline__ float sel_exp(float x, float top) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fmul_rn(__fsub_rn(x, top), 1.4426950408889634f)));
     return y;
 }
+
+// exp(x - top), 1 for nothing on both sides
+__device__ __forceinline__ float sel_scale(float x, float top) { return x == top ? 1.0f : sel_exp(x, top); }
 
 // log(s) for a positive normal s, to 1e-12: with s = 2^e f and c near 1 / f in steps of 1/256
 // (64 intervals of f, Tang's table method), log s = e log 2 - log c + log(1 + r), r = f c - 1, |r| <
@@ -179,6 +200,7 @@ struct SelP {
     const float *logits;
     size_t logits_stride;
     int requests, beams, parts, codebook, eos, has_eos;
+    double near;                   // 2 sel_eps
     const int *allow_eos;
     const float *score;
     const unsigned *done, *live;
@@ -190,21 +212,51 @@ __device__ __forceinline__ void copy_async(float4 *to, const float4 *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
-// Maximum and sum of exponentials of the tokens a thread has seen; NaN is passed over by the
-// maximum and shows in the sum.  `most` receives the pieces' maxima.
+// The tokens a thread has seen: their maximum `top` and the sum of exp(x - base).  `base` follows the
+// maximum in steps above SEL_SLACK only, so a term is scaled to another base once per SEL_SLACK that it
+// lies below the maximum, at most.  NaN is passed over by the maximum and shows in the sum.  `most`
+// receives the pieces' maxima.  Returns what sums formed before have to be scaled by.
+struct SelSeen { float top, base, sum; };
+__device__ __forceinline__ SelSeen sel_none() { return SelSeen{-INFINITY, -INFINITY, 0.0f}; }
+
 template <int N>
-__device__ __forceinline__ void sel_take(const float4 (&x)[N], float (&most)[N], float &top, float &sum) {
-    float m = top;
+__device__ __forceinline__ float sel_take(const float4 (&x)[N], float (&most)[N], SelSeen &s) {
+    float scaled = 1.0f;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         most[u] = fmaxf(fmaxf(x[u].x, x[u].y), fmaxf(x[u].z, x[u].w));
-        m = fmaxf(m, most[u]);
+        s.top = fmaxf(s.top, most[u]);
     }
-    if (m > top) { sum = __fmul_rn(sum, sel_exp(top, m)); top = m; }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    if (s.top > s.base + SEL_SLACK) {
+        scaled = sel_exp(s.base, s.top);
+        s.sum = __fmul_rn(s.sum, scaled);
+        s.base = s.top;
+    }
+    const float ref = s.base == -INFINITY ? 0.0f : s.base;
+    float part = 0.0f;
 #pragma unroll
     for (int u = 0; u < N; ++u)
-        sum += (sel_exp(x[u].x, ref) + sel_exp(x[u].y, ref)) + (sel_exp(x[u].z, ref) + sel_exp(x[u].w, ref));
+        part += (sel_exp(x[u].x, ref) + sel_exp(x[u].y, ref)) + (sel_exp(x[u].z, ref) + sel_exp(x[u].w, ref));
+    s.sum += part;
+    return scaled;
+}
+
+// How far a log-sum may be off.  With u = 2^-24, per term relative to itself: the difference to a
+// base or maximum, its product with log2 e and that constant are off by 2.25 u times the difference,
+// ex2.approx by 4 u.  A term's factors (to its thread's base, the warp's maximum, the part's, the
+// row's) are four such steps, whose differences add up to the term's distance from the row's maximum
+// and twice SEL_SLACK, and 5 u for each change of the base; weighted by the terms the distance is at
+// most the entropy, log(tokens).  The 32-bit sums of a turn are 7 deep, those of turns 2 more than
+// there are.  Up to 2^18 tokens 2^-16.8 in all.
+double sel_eps(size_t tokens) {
+    const double distance = log((double)tokens + 1.0), half = (double)(tokens / (8u * SEL_HELD * SEL_THREADS)) + 1.0;
+    return (2.25 * (distance + 2.0 * SEL_SLACK) + 16.0 + 5.0 * (distance / SEL_SLACK + 1.0) + 9.0 + fmin(2.0 * half, fmax(half, SEL_FOLD))) / 16777216.0;
+}
+
+// Order-preserving bits of a score, 0 for none (NaN and -inf among them).
+__device__ __forceinline__ unsigned long long sel_order(double c) {
+    const long long bits = __double_as_longlong(c + 0.0);
+    return c > -INFINITY ? (unsigned long long)(bits < 0 ? ~bits : bits | (1ll << 63)) : 0ull;
 }
 
 // The keys of the tokens that reach the bound into the list: `most` are the pieces' maxima, piece
@@ -246,6 +298,137 @@ __device__ __forceinline__ float sel_bound(SelScratch &w, float top, int beams) 
     }
     __syncthreads();
     return w.bound;
+}
+
+// Continuation threadIdx.x of the request, at most 16 x 16, of beam b: its score as an ordered integer.
+__device__ __forceinline__ void sel_score(SelSmem &sm, int beams, int parts, int b, unsigned done, int eos, float score, double near) {
+    const int part = threadIdx.x / beams, k = threadIdx.x - part * beams, to = part * SEL_PAD + k;
+    unsigned long long key;
+    double c;
+    if (done >> b & 1u) {
+        key = part == b * parts && k == 0 ? sel_key(0.0f, (unsigned)eos) : 0ull;
+        c = score;
+    } else {
+        key = sm.part[part].key[k];
+        c = (double)score + ((double)sel_logit(key) - sm.part[b * parts].lse);
+    }
+    sm.key[to] = key;
+    sm.score[to] = c;
+    sm.order[to] = key != 0ull ? sel_order(c) : 0ull;
+    sm.near[to] = key != 0ull ? (unsigned)(sel_order(c + near) >> 32) : 0u;
+}
+
+// The lists fall, so the best continuation left is the best of their heads: one warp takes `beams`
+// of them, a list per lane, and returns how many there are.  `close`: with LOOK the beams that come
+// within `near` of a pick of another one, else the lanes whose list's head may.
+template <bool LOOK>
+__device__ __forceinline__ int sel_merge(SelSmem &sm, int beams, int parts, double near, unsigned &close) {
+    const int lane = threadIdx.x, lists = beams * parts, last = lane * SEL_PAD + beams;    // behind a list lies a 0
+    int at = lane * SEL_PAD, found = 0;
+    unsigned long long head = lane < lists ? sm.order[at] : 0ull, next = lane < lists ? sm.order[at + 1] : 0ull;
+    unsigned head_near = lane < lists ? sm.near[at] : 0u, next_near = lane < lists ? sm.near[at + 1] : 0u;
+    bool beside = false;
+    close = 0u;
+    for (; found < beams; ++found) {
+        const unsigned high = __reduce_max_sync(MB_FULL, (unsigned)(head >> 32));
+        if (high == 0u) break;                         // nothing is left (an order's first bits are not 0)
+        unsigned best = __ballot_sync(MB_FULL, (unsigned)(head >> 32) == high);
+        if (best & (best - 1)) {
+            const bool first = (unsigned)(head >> 32) == high;
+            const unsigned low = __reduce_max_sync(MB_FULL, first ? (unsigned)head : 0u);
+            best = __ballot_sync(MB_FULL, first && (unsigned)head == low);
+            // equal scores: the lower beam, which is the lower list; parts of one beam by their keys
+            int winner = __ffs(best) - 1;
+            for (unsigned more = best & (best - 1); parts > 1 && more != 0u; more &= more - 1) {
+                const int other = __ffs(more) - 1;
+                const unsigned long long a = sm.key[__shfl_sync(MB_FULL, at, winner)], o = sm.key[__shfl_sync(MB_FULL, at, other)];
+                if (other / parts == winner / parts && o > a) winner = other;
+            }
+            best = 1u << winner;
+        }
+        const bool won = best >> lane & 1u;
+        if (LOOK) {
+            const double least = sm.score[__shfl_sync(MB_FULL, at, __ffs(best) - 1)] - near;
+            const unsigned who = __reduce_or_sync(MB_FULL, head != 0ull && sm.score[at] >= least ? 1u << (lane / parts) : 0u);
+            if (who & (who - 1)) close |= who;
+        } else {
+            beside = beside || (!won && head_near >= high);
+        }
+        if (won) sm.taken[found] = at;
+        head = won ? next : head;
+        head_near = won ? next_near : head_near;
+        at += won;
+        next = sm.order[lane < lists ? min(at + 1, last) : 0];
+        next_near = sm.near[lane < lists ? min(at + 1, last) : 0];
+    }
+    __syncwarp();
+    if (!LOOK) close = __ballot_sync(MB_FULL, beside);
+    return found;
+}
+
+// exp(d) for -700 <= d <= 0 in 64 bits, to 1e-15: with d = (64 k + j) log(2) / 64 + r, |r| < 0.0055, it is
+// 2^k 2^(j/64) e^r (Tang's table method), e^r - 1 by its series to r^5.  `table` holds 2^(j/64).
+constexpr int SEL_POWERS = 64;
+__device__ __forceinline__ double sel_exp64(double d, const double *table) {
+    constexpr double ROUND = 6755399441055744.0;       // 3 * 2^51: the sum's last bits are the rounded product
+    const double t = fma(d, SEL_POWERS / 0.6931471805599453, ROUND), r = fma(t - ROUND, -0.6931471805599453 / SEL_POWERS, d);
+    const int n = __double2loint(t);
+    const double e = r * fma(r, fma(r, fma(r, fma(r, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0);
+    const double power = table[n & (SEL_POWERS - 1)], y = fma(power, e, power);
+    return __hiloint2double(__double2hiint(y) + (n >> 6 << 20), __double2loint(y));
+}
+
+struct SelRow { const float *row; size_t stride; int codebook, eos; bool allow; };
+
+// Some pick may have come close to another beam's continuation: the log-sums of the beams that did, in
+// 64 bits.  Tokens go to threads by their index, so a sum depends on the logits alone.  All threads of
+// the CTA; false where none came close after all.  Bound by its 64-bit arithmetic: two rows of 2,016
+// add 6 us to the call, of 50,000 33 us, sixteen 230.  With normal logits one call in 60 of 64
+// requests x 8 beams x 2,016 has such a pair, and one in 20 of 24 x 16 x 50,000.
+template <int NTHREADS>
+__device__ __noinline__ bool sel_refine(SelSmem &sm, int beams, int parts, unsigned done, double near, SelRow q) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int SEL_BATCH = 8;
+    double *wsum = sm.work[0].wsum, *table = reinterpret_cast<double *>(sm.work[0].reach);
+    if (tid >= NTHREADS - SEL_POWERS) table[tid - (NTHREADS - SEL_POWERS)] = exp2((double)(tid - (NTHREADS - SEL_POWERS)) / SEL_POWERS);
+    if (warp == 0) {
+        unsigned close;
+        sel_merge<true>(sm, beams, parts, near, close);
+        if (lane == 0) sm.close_beams = close;
+    }
+    __syncthreads();
+    const unsigned close = sm.close_beams;
+    for (int b = 0; b < beams; ++b) {
+        if (!((close & ~done) >> b & 1u)) continue;
+        const float *row = q.row + (size_t)b * q.stride;
+        SelPart *of = sm.part + b * parts;
+        float m = -INFINITY;
+        for (int j = 0; j < parts; ++j) m = fmaxf(m, of[j].top);
+        double sum = 0.0;
+        const auto take = [&](float x) {               // NaN and what is below 1e-300 add nothing
+            const double d = (double)x - (double)m;
+            sum += d > -690.0 ? sel_exp64(d, table) : 0.0;
+        };
+        if (tid == 0 && q.allow) take(row[q.eos]);
+        for (int t0 = tid; t0 < q.codebook; t0 += SEL_BATCH * NTHREADS) {
+            float x[SEL_BATCH];
+#pragma unroll
+            for (int u = 0; u < SEL_BATCH; ++u) x[u] = t0 + u * NTHREADS < q.codebook ? row[t0 + u * NTHREADS] : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < SEL_BATCH; ++u) take(x[u]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(MB_FULL, sum, o);
+        __syncthreads();                               // the sums before are read
+        if (lane == 0) wsum[warp] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < NTHREADS / 32; ++w) sum += wsum[w];
+            of->lse = (double)m + log(sum);
+        }
+    }
+    __syncthreads();
+    return close != 0u;
 }
 
 // FIT: parts of at most SEL_HELD pieces per thread.
@@ -336,20 +519,21 @@ __global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 :
         const float4 *at = r.base + r.whole_from + tid;            // this thread's next piece
         unsigned token = (unsigned)(r.origin + 4 * (r.whole_from + tid));
         float4 x[SEL_HELD];
-        float most[SEL_HELD], beside_most[2], bound, top = -INFINITY, sum = 0.0f;
+        float most[SEL_HELD], beside_most[2], bound;
+        SelSeen seen = sel_none();
         if (FIT) {
 #pragma unroll
             for (int u = 0; u < SEL_HELD; ++u) {
                 x[u] = no_tokens();
                 if (tid + u * NT < whole) x[u] = at[u * NT];
             }
-            sel_take(x, most, top, sum);
-            sel_take(beside, beside_most, top, sum);
-            bound = sel_bound<NT>(w, top, beams);
+            sel_take(x, most, seen);
+            sel_take(beside, beside_most, seen);
+            bound = sel_bound<NT>(w, seen.top, beams);
             const unsigned tokens[SEL_HELD] = {token, token + 4 * NT, token + 8 * NT, token + 12 * NT};
             sel_reach(w, x, most, tokens, bound);
         } else {
-            sel_take(beside, beside_most, top, sum);
+            sel_take(beside, beside_most, seen);
             bound = INFINITY;
             for (int turn = 0, left = whole; left > 0; ++turn, left -= TURN, token += 4 * TURN) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(SEL_DEPTH - 1) : "memory");
@@ -361,27 +545,41 @@ __global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 :
                     for (int u = 0; u < SEL_HELD; ++u)
                         if (tid + u * NT >= left) x[u] = no_tokens();
                 ask();
-                sel_take(x, most, top, sum);
-                if ((turn & (turn + 1)) == 0) bound = sel_bound<NT>(w, top, beams);
+                sel_take(x, most, seen);
+                if ((turn & (turn + 1)) == 0) {
+                    bound = sel_bound<NT>(w, seen.top, beams);
+                    if (turn >= SEL_FOLD - 1) {
+                        const double before = turn >= SEL_FOLD ? sm.folded[tid] * (double)sel_scale(sm.folded_base[tid], seen.base) : 0.0;
+                        sm.folded[tid] = before + (double)seen.sum;
+                        sm.folded_base[tid] = seen.base;
+                        seen.sum = 0.0f;
+                    }
+                }
                 const unsigned tokens[SEL_HELD] = {token, token + 4 * NT, token + 8 * NT, token + 12 * NT};
                 sel_reach(w, x, most, tokens, bound);
             }
-            if (whole <= 0) bound = sel_bound<NT>(w, top, beams);
+            if (whole <= 0) bound = sel_bound<NT>(w, seen.top, beams);
         }
         const unsigned beside_tokens[2] = {(unsigned)(r.origin + 4 * edge), (unsigned)p.eos};
         sel_reach(w, beside, beside_most, beside_tokens, bound);
-        if (sum != sum) {              // NaN among the logits, or +inf: the sum again without them
-            sum = 0.0f;
-            top = -INFINITY;
+        double sum = (double)seen.sum;
+        if (!FIT && whole > (SEL_FOLD - 1) * TURN) sum += sm.folded[tid] * (double)sel_scale(sm.folded_base[tid], seen.base);
+        if (sum != sum) {              // NaN among the logits, or +inf: the sum again without NaN
+            sum = 0.0;
+            seen = sel_none();
+            const auto add = [&](float scaled) {
+                sum = sum * (double)scaled + (double)seen.sum;
+                seen.sum = 0.0f;
+            };
             for (int v = tid; v < whole; v += NT, at += NT) {
                 const float4 y[1] = {drop_nan(*at)};
                 float unused[1];
-                sel_take(y, unused, top, sum);
+                add(sel_take(y, unused, seen));
             }
-            sel_take(beside, beside_most, top, sum);
+            add(sel_take(beside, beside_most, seen));
         }
-        const float wtop = warp_max(top);
-        double wsum = top == -INFINITY ? 0.0 : (double)__fmul_rn(sum, top == wtop ? 1.0f : sel_exp(top, wtop));
+        const float wtop = warp_max(seen.top);
+        double wsum = seen.top == -INFINITY ? 0.0 : sum * (double)sel_scale(seen.base, wtop);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) wsum += __shfl_xor_sync(MB_FULL, wsum, o);
         if (lane == 0) { w.wtop[warp] = wtop; w.wsum[warp] = wsum; }
@@ -396,7 +594,7 @@ __global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 :
         if (warp == WARPS - 1 - q) {   // the sum of the part
             const float t = lane < WARPS ? w.wtop[lane] : -INFINITY;
             const float m = warp_max(t);
-            double all = t == -INFINITY ? 0.0 : w.wsum[lane] * (double)(t == m ? 1.0f : sel_exp(t, m));
+            double all = t == -INFINITY ? 0.0 : w.wsum[lane] * (double)sel_scale(t, m);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(MB_FULL, all, o);
             if (lane == 0) {
@@ -454,75 +652,48 @@ __global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 :
     cluster.sync();
     if (rank != 0) return;
 
-    // the continuations of all parts, at most 16 x 16, and their scores as ordered integers
     if (tid < beams && parts > 1 && !(done >> tid & 1u)) {
         SelPart *of = sm.part + tid * parts;
         float m = -INFINITY;
         for (int j = 0; j < parts; ++j) m = fmaxf(m, of[j].top);
         double all = 0.0;
         for (int j = 0; j < parts; ++j)
-            if (of[j].top != -INFINITY) all += of[j].sum * (double)(of[j].top == m ? 1.0f : sel_exp(of[j].top, m));
+            if (of[j].top != -INFINITY) all += of[j].sum * (double)sel_scale(of[j].top, m);
         of[0].lse = all >= 0.5 ? (double)m + sel_log(all) : (double)NAN;
     }
     if (parts > 1) __syncthreads();
-    if (tid < beams * parts) sm.order[tid * SEL_PAD + beams] = 0ull;
-    if (tid < n) {
-        const int part = tid / beams, k = tid - part * beams, b = mine, to = part * SEL_PAD + k;
-        unsigned long long key;
-        double c;
-        if (done >> b & 1u) {
-            key = part == b * parts && k == 0 ? sel_key(0.0f, (unsigned)p.eos) : 0ull;
-            c = score;
-        } else {
-            key = sm.part[part].key[k];
-            c = (double)score + ((double)sel_logit(key) - sm.part[b * parts].lse);
-        }
-        sm.key[to] = key;
-        sm.score[to] = c;
-        const long long bits = __double_as_longlong(c + 0.0);
-        // 0: no candidate (NaN and -inf among them)
-        sm.order[to] = key != 0ull && c > -INFINITY ? (unsigned long long)(bits < 0 ? ~bits : bits | (1ll << 63)) : 0ull;
+    if (tid < beams * parts) {
+        sm.order[tid * SEL_PAD + beams] = 0ull;
+        sm.near[tid * SEL_PAD + beams] = 0u;
+    }
+    if (tid < n) sel_score(sm, beams, parts, mine, done, p.eos, score, p.near);
+    __syncthreads();
+    const auto store = [&](int found_all) {            // first `beams` threads
+        const int to = request * beams + tid;
+        const bool alive = tid < found_all;
+        const int from = alive ? sm.taken[tid] : 0;
+        const unsigned t = alive ? sel_token(sm.key[from]) : 0u;
+        p.score_out[to] = alive ? (float)sm.score[from] : -INFINITY;
+        p.token[to] = t;
+        p.parent[to] = alive ? (unsigned)(from / SEL_PAD / parts) : (unsigned)tid;         // dead: stays where it is
+        if (p.done_out != nullptr) p.done_out[to] = alive && t == (unsigned)p.eos ? 1u : 0u;
+    };
+    unsigned close;
+    if (warp == 0) {
+        const int picked = sel_merge<false>(sm, beams, parts, p.near, close);
+        if (tid < beams) store(picked);                // as a rule these stay
+        if (tid == 0) sm.close = close;
     }
     __syncthreads();
-    // The lists fall, so the best continuation left is the best of their heads: one warp takes
-    // `beams` of them, a list per lane.
-    if (tid >= 32) return;
-    const int lists = beams * parts, last = tid * SEL_PAD + beams;     // behind a list lies a 0
-    int at = tid * SEL_PAD, found_all = 0;
-    unsigned long long head = tid < lists ? sm.order[at] : 0ull, next = tid < lists ? sm.order[at + 1] : 0ull;
-    for (; found_all < beams; ++found_all) {
-        const unsigned high = __reduce_max_sync(MB_FULL, (unsigned)(head >> 32));
-        if (high == 0u) break;                         // nothing is left (an order's first bits are not 0)
-        unsigned best = __ballot_sync(MB_FULL, (unsigned)(head >> 32) == high);
-        if (best & (best - 1)) {
-            const bool first = (unsigned)(head >> 32) == high;
-            const unsigned low = __reduce_max_sync(MB_FULL, first ? (unsigned)head : 0u);
-            best = __ballot_sync(MB_FULL, first && (unsigned)head == low);
-            // equal scores: the lower beam, which is the lower list; parts of one beam by their keys
-            int winner = __ffs(best) - 1;
-            for (unsigned more = best & (best - 1); parts > 1 && more != 0u; more &= more - 1) {
-                const int other = __ffs(more) - 1;
-                const unsigned long long a = sm.key[__shfl_sync(MB_FULL, at, winner)], o = sm.key[__shfl_sync(MB_FULL, at, other)];
-                if (other / parts == winner / parts && o > a) winner = other;
-            }
-            best = 1u << winner;
-        }
-        const bool won = best >> tid & 1u;
-        if (won) sm.taken[found_all] = at;
-        head = won ? next : head;
-        at += won;
-        next = sm.order[tid < lists ? min(at + 1, last) : 0];
+    if (sm.close == 0u) return;
+    const SelRow rows = {p.logits + (size_t)request * beams * p.logits_stride, p.logits_stride, p.codebook, p.eos, allow};
+    if (!sel_refine<NT>(sm, beams, parts, done, p.near, rows)) return;
+    if (tid < n) sel_score(sm, beams, parts, mine, done, p.eos, score, p.near);
+    __syncthreads();
+    if (warp == 0) {
+        const int picked = sel_merge<false>(sm, beams, parts, p.near, close);
+        if (tid < beams) store(picked);
     }
-    __syncwarp();
-    if (tid >= beams) return;
-    const int to = request * beams + tid;
-    const bool alive = tid < found_all;
-    const int from = alive ? sm.taken[tid] : 0;
-    const unsigned t = alive ? sel_token(sm.key[from]) : 0u;
-    p.score_out[to] = alive ? (float)sm.score[from] : -INFINITY;
-    p.token[to] = t;
-    p.parent[to] = alive ? (unsigned)(from / SEL_PAD / parts) : (unsigned)tid;         // dead: stays where it is
-    if (p.done_out != nullptr) p.done_out[to] = alive && t == (unsigned)p.eos ? 1u : 0u;
 }
 
 // ------------------------------------------------------------------------ reordering
@@ -656,6 +827,7 @@ extern "C" int mb_beam_select(const mb_beam_select_args *a, mb_stream stream) {
     p.score = a->score;
     p.done = a->done;
     p.live = a->live;
+    p.near = 2.0 * sel_eps(a->codebook_size);
     p.score_out = a->score_out;
     p.token = a->token;
     p.parent = a->parent;

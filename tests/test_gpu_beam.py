@@ -645,6 +645,53 @@ def test_select_orders_and_ties(be, order):
         check_select(be, logits, score, None, vocab - 1, vocab - 1, np.array([1, 0]))
 
 
+@pytest.mark.parametrize("beams, vocab", [(2, 2016), (16, 2016), (3, 257), (2, 20011), (9, 20011), (16, 40960)])
+def test_select_of_equal_beams_at_every_alignment(be, beams, vocab):
+    """Beams with equal rows and scores are equal, wherever their rows begin: the lower one comes
+    first, place by place."""
+    r = np.random.default_rng(vocab + beams)
+    requests = 12 if vocab < 4096 else 2
+    for stride in (vocab, vocab + 1, vocab + 2, vocab + 3):
+        rows = r.normal(0, 2, (requests, 1, vocab)).astype(np.float32)
+        check_select(be, np.repeat(rows, beams, 1), np.repeat(-20 * r.random((requests, 1)), beams, 1), None, vocab, vocab, None,
+                     stride=stride, offset=stride % 3)
+
+
+@pytest.mark.parametrize("vocab", [2016, 20011])
+def test_select_keeps_the_order_of_close_beams(be, vocab):
+    """Beams whose continuations are 1e-9 or 4e-10 apart, by their scores (the rows hold the same
+    logits in another order, so the log-sums are equal) or by one small logit of a row: the order
+    is that of the definition in 64 bits, whose own rounding is below 1e-13."""
+    r = np.random.default_rng(vocab)
+    for trial in range(8 if vocab < 4096 else 2):
+        row = r.normal(0, 2, vocab).astype(np.float32)
+        logits = np.stack([row, r.permutation(row)] * 2)[None]
+        score = np.float32([[-1e-3, -1e-3 + 1e-9, -2e-3 + 1e-9, -2e-3]])
+        if trial % 2:                                        # one of the smallest logits grows: its beam falls by 1.6e-9
+            at = np.argsort(logits[0, 2])[vocab // 200]
+            whole = np.exp(row.astype(np.float64)).sum()
+            logits[0, 2, at] = np.log(np.exp(np.float64(logits[0, 2, at])) + 1.6e-9 * whole)
+        best = np.sort(ref.select(logits, score, np.zeros((1, 4), int), vocab, vocab, np.ones(1))[0][0])
+        assert np.diff(best).min() > 5e-11                   # the definition itself has no doubt
+        check_select(be, logits, score, None, vocab, vocab, None, stride=vocab + 1)
+
+
+def test_select_of_rows_beyond_the_turns_that_32_bits_sum(be):
+    """Equal beams of 300,001 logits, 37 turns of a thread, that rise by 300 along the vocabulary, so
+    that the sums' base moves; and rows most of whose threads see nothing, or NaN, for 32 turns."""
+    vocab = 300001
+    r = np.random.default_rng(9)
+    row = (np.arange(vocab) / 1000.0 + r.normal(0, 1, vocab)).astype(np.float32)
+    empty = np.where(np.arange(vocab) % 4096 < 5, row, -np.inf).astype(np.float32)
+    odd = np.where(np.arange(vocab) % 4096 < 5, row, np.nan).astype(np.float32)
+    done = np.zeros((1, 9), np.int64)
+    done[0, 2:] = 1
+    score = np.full((1, 9), -np.inf)
+    score[0, :2] = -3.0
+    for x in (row, empty, odd):
+        check_select(be, np.repeat(x[None, None], 9, 1), score, done, vocab - 3, vocab - 1, np.array([0]))
+
+
 def test_select_with_gathered_large_logits(be):
     """All candidates in the pieces of fewer threads than there are places, thousands of them."""
     vocab = 40960
