@@ -497,11 +497,12 @@ int mynah_b200_codec_time(void *codec, const unsigned *codes, size_t frames, int
  *   mynah_b200_beam_reorder    gives the picked beams their parents' own rows
  *
  * Pointers named dev_* are memory of the backend's device, from mynah_cuda_dev_alloc or any
- * other allocation there.  The calls enqueue on the backend's stream and return; they neither
- * allocate nor synchronize, so they may be captured into a CUDA graph, and they leave the
- * calling thread's current device as it was.  Lengths, slots, prefixes, parents and the live
- * counts are read on the device when the work runs: a captured graph follows their current
- * values.  Every operator computes the same in strict and in fast mode. */
+ * other allocation there; arrays of floats and of 32-bit integers start on 4 bytes.  The calls
+ * enqueue on the backend's stream and return; they neither allocate nor synchronize, so they may
+ * be captured into a CUDA graph, and they leave the calling thread's current device as it was.
+ * Lengths, slots, prefixes, parents and the live counts are read on the device when the work
+ * runs: a captured graph follows their current values.  Every operator computes the same in
+ * strict and in fast mode. */
 
 /* K and V rows of `slots` slots: slot_stride elements apart, `capacity` rows each,
  * row_stride apart, `width` elements per row.  type is MYNAH_B200_F32 or MYNAH_B200_F16.

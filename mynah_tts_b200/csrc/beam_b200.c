@@ -31,6 +31,12 @@ static int refuse(const char *message, char *error, size_t cap) {
 #define MB_LANE_ROWS_MAX ((size_t)1 << 30)
 
 static int aligned4(const void *p) { return ((uintptr_t)p & 3u) == 0; }
+/* Arrays of 32-bit values; NULL, for one left out, is aligned. */
+static int all_aligned4(const void *const *arrays, size_t n) {
+    for (size_t i = 0; i < n; ++i)
+        if (!aligned4(arrays[i])) return 0;
+    return 1;
+}
 static int aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 /* 0 when rows of `width` elements can be walked in 16-byte pieces. */
@@ -85,6 +91,9 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
     if (a->dev_qkv == NULL || a->qkv_stride < 3u * width || a->dev_length == NULL || a->dev_out == NULL ||
         a->out_stride < width || !aligned4(a->dev_qkv) || !aligned4(a->dev_out))
         return refuse("invalid lane attention buffers", error, cap);
+    const void *words[] = {a->dev_slot, a->dev_length, a->dev_live};
+    if (!all_aligned4(words, sizeof(words) / sizeof(words[0])))
+        return refuse("lane attention arrays must be 4-byte aligned", error, cap);
     if (a->dev_slot == NULL && a->cache.slots < a->lanes)
         return refuse("fewer slots than lanes", error, cap);
     size_t prefix_capacity = 0;
@@ -93,6 +102,9 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
         if (a->prefixes > MB_LANES_MAX || a->dev_prefix_k == NULL || a->dev_prefix_v == NULL || a->dev_prefix_length == NULL ||
             prefix_capacity == 0 || prefix_capacity > 0x7fffffffu || a->prefix_row_stride > 0x1fffffffu)
             return refuse("invalid lane attention prefixes", error, cap);
+        const void *of_prefixes[] = {a->dev_prefix_length, a->dev_lane_prefix};
+        if (!all_aligned4(of_prefixes, sizeof(of_prefixes) / sizeof(of_prefixes[0])))
+            return refuse("lane attention arrays must be 4-byte aligned", error, cap);
         if (a->prefix_row_stride < width || a->prefix_row_stride % per != 0 || a->prefix_stride % per != 0 ||
             (a->prefixes > 1 && a->prefix_stride == 0) || !aligned16(a->dev_prefix_k) || !aligned16(a->dev_prefix_v))
             return refuse("prefix rows must be 16-byte aligned and prefix_row_stride at least the width", error, cap);
@@ -157,6 +169,10 @@ int mynah_b200_beam_select(void *state, const mynah_b200_beam_select_args *a, ch
     if (a->dev_logits == NULL || a->dev_score == NULL || a->dev_score_out == NULL || a->dev_token == NULL ||
         a->dev_parent == NULL || a->dev_token == a->dev_parent || ((uintptr_t)a->dev_logits & 3u) != 0)
         return refuse("invalid beam selection buffers", error, cap);
+    const void *words[] = {a->dev_allow_eos, a->dev_score,  a->dev_done,   a->dev_live,
+                           a->dev_score_out, a->dev_token, a->dev_parent, a->dev_done_out};
+    if (!all_aligned4(words, sizeof(words) / sizeof(words[0])))
+        return refuse("beam selection arrays must be 4-byte aligned", error, cap);
     mb_beam_select_args m;
     memset(&m, 0, sizeof(m));
     m.logits = a->dev_logits;
@@ -194,6 +210,9 @@ int mynah_b200_beam_reorder(void *state, const mynah_b200_beam_reorder_args *a, 
     if (check_cache(&a->cache, 1, error, cap) != 0) return -1;
     if (a->dev_parent == NULL || a->dev_length == NULL || a->dev_length_out == a->dev_length)
         return refuse("invalid beam reorder buffers", error, cap);
+    const void *words[] = {a->dev_slot, a->dev_parent, a->dev_length, a->dev_length_out, a->dev_live};
+    if (!all_aligned4(words, sizeof(words) / sizeof(words[0])))
+        return refuse("beam reorder arrays must be 4-byte aligned", error, cap);
     if (a->dev_slot == NULL && a->cache.slots < a->requests * a->beams)
         return refuse("fewer slots than lanes", error, cap);
     mb_beam_reorder_args m;

@@ -112,6 +112,20 @@ def test_beam_reorder_refuses(change, cache):
     assert refusal(capi.lib().mynah_b200_beam_reorder, reorder(cache, **change))
 
 
+def test_arrays_that_are_not_aligned_are_refused():
+    """The kernels read and write them as 32-bit values, which a device faults on elsewhere."""
+    lib = capi.lib()
+    for fn, make, names in (
+            (lib.mynah_b200_lane_attention, attention, "dev_slot dev_length dev_prefix_length dev_lane_prefix dev_live"),
+            (lib.mynah_b200_beam_select, select,
+             "dev_allow_eos dev_score dev_done dev_live dev_score_out dev_token dev_parent dev_done_out"),
+            (lib.mynah_b200_beam_reorder, reorder, "dev_slot dev_parent dev_length dev_length_out dev_live")):
+        for name in names.split():
+            for off in (1, 2, 3):
+                said = refusal(fn, make(**{name: 4 * A + off}))
+                assert "4-byte aligned" in said, (name, said)
+
+
 def test_decoder_reorder_refuses_without_a_decoder():
     err = C.create_string_buffer(capi.ERR_CAP)
     one = (C.c_uint * 1)(0)
