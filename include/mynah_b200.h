@@ -536,6 +536,8 @@ typedef struct {
  * A prefix that enough lanes share is multiplied on the tensor cores, once for 128 lanes; the
  * environment, read when the backend is opened, overrides the choice: MYNAH_B200_LANE_TILES=0
  * (and MYNAH_B200_NO_TC=1) never, =1 for any 8 lanes.  Results agree to 32-bit rounding.
+ * Waits on the device are bounded: one that runs out makes the call's outputs stale and the next
+ * mynah_cuda_sync report it.  MYNAH_B200_LANE_POLLS, read likewise, shortens them (tests).
  *
  * Limits: 1 .. 1024 lanes, 1 .. 64 heads, head_width up to 128 in multiples of 16 bytes of the
  * cache's type, lanes * (capacity + prefix_capacity) <= 2^30. */

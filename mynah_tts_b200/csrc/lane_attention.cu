@@ -43,6 +43,7 @@ struct LaneP {
     float *out;
     size_t out_stride;
     int *status;
+    unsigned polls;                // of a barrier, before a wait gives up
     // workspace
     unsigned *offset;              // [lanes + 1] rows of the lanes counted on, then the run length
     float2 *stat;                  // [part][heads] maximum, sum
@@ -247,6 +248,12 @@ __device__ void lane_schedule(const LaneP &p, unsigned *off, unsigned *end, unsi
 // TB/s; the others are the schedule (2), the first rows' latency (2), uneven ends (3) and the merge
 // (5).  Four steps of 8 rows instead of two of 16 save 1 us, but 8 rows at a time cost 4 to 15% wherever
 // rows come from L2 or one CTA has an SM to itself.
+//
+// A wait that runs out (the copies take seconds: the device is in trouble) ends the launch in bounded
+// time: the warp's lane is joined once more, so that no warp is missing at a barrier, and behind
+// the barrier all warps of the CTA leave; without barriers each leaves alone.  A warp that has
+// left empties no step, so the bringing warp and the others run out in turn.  The copies under
+// way have landed, or have been waited for once more, before the CTA ends.
 constexpr int ROWS_DEPTH = 2;
 constexpr size_t ROWS_STAGE = 50u * 1024u;       // bytes of a step, at most
 
@@ -271,6 +278,7 @@ template <typename T, int LPR, bool FULL>
 __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
     extern __shared__ uint4 sm_rows_dyn[];
     __shared__ unsigned s_run, s_end[FEW_LANES];
+    __shared__ volatile int s_lost;              // a warp's wait has run out
     __shared__ float s_acc[WARPS_MAX][MB_LANE_HEAD_WIDTH_MAX];
     __shared__ float2 s_stat[WARPS_MAX];
     __shared__ __align__(8) unsigned long long s_full[ROWS_DEPTH], s_empty[ROWS_DEPTH];
@@ -280,6 +288,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = p.heads_per_cta * p.phases, step = p.step;
     const unsigned plane = (unsigned)(step * p.row_pitch);       // K rows of a stage, then V rows
     if (threadIdx.x == 0) {
+        s_lost = 0;
         for (int i = 0; i < ROWS_DEPTH; ++i) {
             bar_init(&s_full[i], 1u);
             bar_init(&s_empty[i], (unsigned)warps);
@@ -318,7 +327,8 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
         const unsigned bytes = (unsigned)min((size_t)p.row_bytes, (size_t)p.width * sizeof(T) - column);
         const ptrdiff_t own_v = p.v - p.k, shared_v = p.prefix_v - p.prefix_k;      // from a row of K to its row of V
         bool fine = true;
-        for (unsigned steps = 0; at < end && fine; ++b) {
+        unsigned steps = 0;
+        for (; at < end && fine; ++b) {
             if (sm_off[b + 1] <= at) continue;
             unsigned r0 = at - sm_off[b];
             const unsigned last = min(end, end_of(b)) - sm_off[b];
@@ -327,8 +337,9 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
             const char *shared = p.prefix_k + w.prefix * p.prefix_stride * sizeof(T) + column;
             at = min(end, sm_off[b + 1]);
             for (; r0 < last && fine; r0 += step) {
-                if (steps++ >= ROWS_DEPTH) fine = __all_sync(MB_FULL, bar_wait(&s_empty[stage], parity ^ 1u, TC_SPIN));
+                if (steps >= ROWS_DEPTH) fine = __all_sync(MB_FULL, bar_wait(&s_empty[stage], parity ^ 1u, p.polls));
                 if (!fine) break;
+                ++steps;
                 const unsigned n = min((unsigned)step, last - r0);
                 if (lane == 0) bar_expect(&s_full[stage], 2u * n * bytes);
                 __syncwarp();
@@ -345,6 +356,8 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
             }
         }
         if (!fine && lane == 0) atomicOr(p.status, 2);
+        for (unsigned i = steps - min(steps, (unsigned)ROWS_DEPTH); i < steps; ++i)       // whoever still reads them
+            bar_wait(&s_full[i % ROWS_DEPTH], i / ROWS_DEPTH & 1u, TC_SPIN);
         last_wait();
         return;
     }
@@ -365,11 +378,12 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
             acc[i] = 0.0f;
         }
         for (unsigned r0 = first; r0 < last; r0 += step) {
-            const bool there = __all_sync(MB_FULL, bar_wait(&s_full[stage], parity, TC_SPIN));
-            if (!there) {                        // the wait has lasted seconds: nothing can be on its way any more
-                if (lane == 0) atomicOr(p.status, 2);
-                last_wait();
-                return;
+            if (!__all_sync(MB_FULL, bar_wait(&s_full[stage], parity, p.polls))) {
+                if (lane == 0) {
+                    atomicOr(p.status, 2);
+                    s_lost = 1;
+                }
+                break;
             }
             const char *from = mine + (size_t)stage * 2u * plane;
             const unsigned most = min((unsigned)step, last - r0) - 1u;
@@ -432,6 +446,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
             for (int o = LPR; o < 32; o <<= 1) a += __shfl_xor_sync(MB_FULL, a, o);
             acc[i] = a;
         }
+        bool lost = __any_sync(MB_FULL, s_lost != 0);      // one answer for the warp
         if (p.phases > 1) {
             if (group == 0) {
                 if (part == 0) s_stat[warp] = make_float2(m, sum);
@@ -439,6 +454,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
                 for (int i = 0; i < 16; ++i) s_acc[warp][((i / PER) * LPR + part) * PER + i % PER] = acc[i];
             }
             asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
+            lost = s_lost != 0;                  // the same for all warps: it is set in front of this barrier only
             if (phase == 0) {
                 float all = m;
                 for (int o = 1; o < p.phases; ++o) all = fmaxf(all, s_stat[warp + o * p.heads_per_cta].x);
@@ -459,6 +475,7 @@ __global__ void __maxnreg__(64) k_lane_rows(LaneP p) {
             }
             asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
         }
+        if (lost) break;
         if (group == 0 && phase == 0 && has_head) {
             const size_t slot = (size_t)(blockIdx.x + b) * p.heads + head;
             if (part == 0) p.stat[slot] = make_float2(m, sum);
@@ -873,6 +890,7 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     p.out = a->out;
     p.out_stride = a->out_stride;
     p.status = a->status;
+    p.polls = a->polls;
     p.offset = reinterpret_cast<unsigned *>(a->workspace + w.offset);
     p.stat = reinterpret_cast<float2 *>(a->workspace + w.stat);
     p.acc = a->workspace + w.acc;

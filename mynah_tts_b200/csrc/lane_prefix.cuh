@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP 
                 mma_commit(&s_bar);
             }
             if (!begun) unscale = mine ? s_unscale[tid] : 1.0f;
-            bool done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
+            bool done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, p.polls));
             parity ^= 1u;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (F16 && done && block + 1 < stop) bring(pk, sk, block + 1);
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(TILE, SLABS == 1 ? 4 : 2) k_lane_prefix(LaneP 
                     }
                 mma_commit(&s_bar);
             }
-            done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, TC_SPIN));
+            done = __all_sync(MB_FULL, bar_wait(&s_bar, parity, p.polls));
             parity ^= 1u;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (F16 && done && block + 1 < stop) bring(pv, sv, block + 1);

@@ -423,8 +423,10 @@ typedef struct {
     int *status;
     int sm_count;
     int tiles;                  /* prefixes on the tensor cores: 0 never, 1 wherever possible, -1 where faster */
+    unsigned polls;             /* of a device barrier, before a wait gives up and sets status */
     unsigned *launched;         /* incremented by the number of kernels the call enqueued */
 } mb_lane_attn_args;
+enum { MB_LANE_POLLS = 1 << 24 };   /* seconds */
 size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count);
 int mb_lane_attention_init(void);
 int mb_lane_attention(const mb_lane_attn_args *args, mb_stream stream);

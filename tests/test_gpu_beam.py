@@ -449,6 +449,35 @@ def test_full_lanes_and_missing_slots_are_left_out_and_reported(be):
     x.check(skipped=(1, 2, 3))
 
 
+@pytest.mark.parametrize("polls", [0, 1, 3])
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("heads, hw, lanes, tiles", [(12, 64, 9, "0"), (2, 64, 9, "0"), (1, 128, 1, "0"), (2, 64, 70, "1")])
+def test_waits_that_run_out_are_reported(be, kind, heads, hw, lanes, tiles, polls):
+    """Waits that give up at once, with warps that share a head's rows and without: the call ends, the
+    next sync says so, and the calls behind it are sound.  A few polls may or may not do."""
+    x = Lanes(be, kind, heads, hw, [300 + 40 * b % 170 for b in range(lanes)], 500, prefix_lengths=[200], seed=14)
+    y = Lanes(be, kind, heads, hw, [300 + 40 * b % 170 for b in range(lanes)], 500, prefix_lengths=[200], seed=15)
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("MYNAH_B200_LANE_TILES", tiles)
+        m.setenv("MYNAH_B200_LANE_POLLS", str(polls))
+        short = Backend("f32")
+    short.set_stream(torch.cuda.current_stream().cuda_stream)
+    x.bind(short)()
+    try:
+        short.sync()
+        said = ""
+        x.check()
+    except MynahB200Error as e:
+        said = str(e)
+        assert "ran out" in said
+    assert said or polls > 0
+    short.sync()                                             # said once
+    short.close()
+    y.bind()()
+    be.sync()
+    y.check()
+
+
 def test_many_lanes(be):
     r = np.random.default_rng(11)
     attend(be, "f16", 1, 32, [int(n) for n in r.integers(0, 12, 1024)], 12, prefix_lengths=[9, 140],
