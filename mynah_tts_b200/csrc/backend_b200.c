@@ -347,8 +347,8 @@ int mynah_b200_open(void **state, int device, int quant, int strict, char *error
         mb_cuda(mb_beam_init(st->beam_clusters), "kernel attributes (beam selection)", error, cap) != 0 ||
         mb_cuda(mb_lane_attention_init(), "kernel attributes (lane attention)", error, cap) != 0 ||
         mb_cuda((int)cudaMalloc((void **)&st->d_token, sizeof(unsigned)), "cudaMalloc", error, cap) != 0 ||
-        mb_cuda((int)cudaMalloc((void **)&st->d_status, sizeof(int)), "cudaMalloc", error, cap) != 0 ||
-        mb_cuda((int)cudaMemset(st->d_status, 0, sizeof(int)), "cudaMemset", error, cap) != 0) {
+        mb_cuda((int)cudaMalloc((void **)&st->d_status, 2u * sizeof(int)), "cudaMalloc", error, cap) != 0 ||
+        mb_cuda((int)cudaMemset(st->d_status, 0, 2u * sizeof(int)), "cudaMemset", error, cap) != 0) {
         mynah_b200_close(st);
         return -1;
     }
@@ -683,11 +683,11 @@ int mynah_cuda_sync(void *state, char *error, size_t cap) {
     MB_TRY(cudaStreamSynchronize(st->stream), "cudaStreamSynchronize");
     /* the seam ops enqueue and return: a bounded device wait that ran out since the last
      * sync is reported here, where the caller collects the step's result */
-    int status = 0;
-    MB_TRY(cudaMemcpy(&status, st->d_status, sizeof(int), cudaMemcpyDeviceToHost), "read status");
-    if (status != 0) {
-        cudaMemset(st->d_status, 0, sizeof(int));
-        mb_set_error(error, cap, mb_status_message(status));
+    int status[2] = {0, 0};
+    MB_TRY(cudaMemcpy(status, st->d_status, sizeof(status), cudaMemcpyDeviceToHost), "read status");
+    if ((status[0] | status[1]) != 0) {
+        cudaMemset(st->d_status, 0, sizeof(status));
+        mb_set_error(error, cap, mb_status_message(status[0] | status[1]));
         return -1;
     }
     mb_clear_error(error, cap);

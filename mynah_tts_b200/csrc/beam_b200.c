@@ -144,7 +144,7 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
     m.out = a->dev_out;
     m.out_stride = a->out_stride;
     m.workspace = a->dev_workspace;
-    m.status = st->d_status;
+    m.status = st->d_status + 1;           /* read by the next sync only: a full lane is no fault of what else runs */
     m.sm_count = st->sm_count;
     m.tiles = st->lane_tiles;
     m.polls = st->lane_polls;

@@ -44,7 +44,7 @@ typedef struct mb_state {
     unsigned *d_counters;
     size_t d_partials_cap, d_counters_cap;
     unsigned *d_token;               /* 1 element */
-    int *d_status;
+    int *d_status;                   /* [0] status bits (mb_status_message), [1] the lane attention's own */
     int sm_count;
     cudaEvent_t timer0, timer1;
     mb_libm_tables libm;             /* strict mode: host-libm correction tables */

@@ -449,6 +449,28 @@ def test_full_lanes_and_missing_slots_are_left_out_and_reported(be):
     x.check(skipped=(1, 2, 3))
 
 
+def test_a_full_lane_is_no_fault_of_what_runs_behind_it(be):
+    """The text encoder and the codec of the same backend read their own status; the lane's report
+    waits for the sync."""
+    from mynah_tts_b200.backend import Codec, TextEncoder
+    other = Backend("f32")
+    encoder = TextEncoder(other, synth.add_encoder(None, synth.TINY_ENCODER, seed=3), synth.TINY_ENCODER)
+    codec = Codec(other, synth.add_codec(None, synth.TINY_CODEC, seed=4), synth.TINY_CODEC, max_frames=4)
+    ids, codes = np.array([1, 2, 3], np.int32), synth.make_codec_codes(synth.TINY_CODEC, 5, 2)
+    want, sound = encoder.encode(ids), codec.decode(codes)
+    for run, result in ((lambda: encoder.encode(ids), want), (lambda: codec.decode(codes), sound)):
+        x = Lanes(other, "f32", 3, 32, [4, 10, 9], 10, seed=10)
+        x.bind()()
+        assert np.array_equal(run(), result)
+        with pytest.raises(MynahB200Error, match="cache is full or its slot"):
+            other.sync()
+        other.sync()
+        x.check(skipped=(1,))
+    encoder.close()
+    codec.close()
+    other.close()
+
+
 @pytest.mark.parametrize("polls", [0, 1, 3])
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("heads, hw, lanes, tiles", [(12, 64, 9, "0"), (2, 64, 9, "0"), (1, 128, 1, "0"), (2, 64, 70, "1")])
