@@ -606,8 +606,10 @@ typedef struct {
     size_t requests, beams;
     const unsigned *dev_slot;          /* [requests * beams], or NULL: lane b owns slot b */
     const unsigned *dev_parent;        /* [requests * beams] beam index within the request */
-    const unsigned *dev_length;        /* [requests * beams] */
-    unsigned *dev_length_out;          /* or NULL */
+    const unsigned *dev_length;        /* [requests * beams] rows that are moved: behind a step's
+                                        * _lane_attention, which appends a row but does not advance
+                                        * lengths, its dev_length + 1 */
+    unsigned *dev_length_out;          /* or NULL; the next step's lengths */
     const unsigned *dev_live;          /* requests in use, or NULL: all */
 } mynah_b200_beam_reorder_args;
 int mynah_b200_beam_reorder(void *state, const mynah_b200_beam_reorder_args *args, char *error, size_t cap);

@@ -2,6 +2,9 @@
 No GPU: every refusal is decided from sizes, strides, alignment and null pointers before the
 backend is used, so a zeroed block stands in for one."""
 import ctypes as C
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -10,6 +13,7 @@ import beam_reference as ref
 from mynah_tts_b200 import capi
 from mynah_tts_b200.backend import Backend
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 STATE = C.create_string_buffer(4096)
 A = 1 << 20                        # an aligned address that no refused call touches
 
@@ -148,6 +152,45 @@ def test_bound_calls_report_a_refusal():
     with pytest.raises(capi.MynahB200Error, match="invalid beam selection"):
         be.beam_select(logits=A, requests=1, beams=1, vocab=4, codebook_size=4, eos_id=4, score=A, score_out=A, token=A,
                        parent=A)
+
+
+def beam_recipe():
+    text = open(os.path.join(ROOT, "INTEGRATION.md")).read()
+    return re.search(r"## 3b.*?```c\n(.*?)```", text, re.S).group(1)
+
+
+def test_the_documented_step_compiles(tmp_path):
+    """INTEGRATION.md's step against the header, with what it takes from its surroundings declared."""
+    source = tmp_path / "step.c"
+    source.write_text("""#include "mynah_b200.h"
+void project_logits(const float *out, float *logits);
+void advance(const unsigned *length, unsigned *grown, size_t n);
+void step(void *state, void *k, void *v, void *pk, void *pv, float *qkv, float *out, float *space, float *logits, float *score,
+          unsigned *length, unsigned *grown, unsigned *context_length, unsigned *token, unsigned *parent, unsigned *done,
+          size_t slots, size_t capacity, size_t width, size_t layers, size_t n, size_t requests, size_t beams, size_t vocab,
+          size_t codebook_size, size_t eos_id, size_t context_rows, char *err, size_t cap) {
+""" + beam_recipe() + "}\n")
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Wextra", "-Werror", "-fsyntax-only", "-I", os.path.join(ROOT, "include"),
+                    str(source)], check=True)
+
+
+def test_the_documented_step_moves_the_newest_row():
+    """Its order of calls and its lengths, with the definitions in the calls' place: a beam that takes
+    another's place goes on from that one's newest row."""
+    recipe = beam_recipe()
+    calls = re.findall(r"^(\w+)\(", recipe, re.M)
+    given = re.search(r"\.dev_length = (\w+), \.dev_length_out = (\w+)", recipe).groups()
+    assert given[1] == "length"
+    k = np.zeros((1, 2, 1, 8, 1))
+    at = {"length": np.array([[3, 3]])}
+    for call in calls:
+        if call == "mynah_b200_lane_attention":
+            k[0, :, 0, 3, 0] = [10.0, 20.0]                  # each lane's new row, behind its three
+        elif call == "advance":
+            at["grown"] = at["length"] + 1
+        elif call == "mynah_b200_beam_reorder":
+            k, at["length"] = ref.reorder(k, np.array([[1, 1]]), at[given[0]])
+    assert k[0, :, 0, 3, 0].tolist() == [20.0, 20.0] and at["length"].tolist() == [[4, 4]]
 
 
 # ---- the definitions against cases worked out by hand
