@@ -53,6 +53,32 @@ def bound(reach, hw, rows):
     return 2 * (2 * dx + 2 * 2.0 ** -22 + rows * u) + 4 * u
 
 
+def drift(q, kk, vv, heads, scale, got):
+    """How far a lane's result `got` is from the definition over rows kk, vv [rows, width], as a
+    sum of squares, and the sum of squares it may reach.  `bound` adds roundings up as if they were all
+    alike; over many outputs they are not, and what is left is far smaller.  With u = 2^-24:
+    * a weight is off by a part d_j of itself, so an output by sum_j d_j w_j (v_j - out): the d_j of
+      the rows go either way, so its square is d^2 sum_j w_j^2 (v_j - out)^2, at most with |v_j| + |out|;
+    * d holds the score's error.  A score is a sum of products of planes, the small ones first, whose
+      sum is below 2^-8 of it; then come up to 8 sums of 16 products (head widths up to 128), each cut
+      to 24 bits of what is summed so far, which is of the size x = log2(e) scale sqrt(sum (q k)^2):
+      sqrt(8) 2 u x / sqrt(3) = 3.3 u x, and as much for what is cut inside a sum of 16: 7 u x;
+    * and the weight's own, 8 u: its approximation 4, its planes 2, its place in the sums 2;
+    * an output is a sum, a quotient and its stored value: 4 u of itself."""
+    u = 2.0 ** -24
+    rows, width = kk.shape
+    qq = q.astype(np.float64).reshape(heads, -1)
+    kk, vv = (t.astype(np.float64).reshape(rows, heads, -1) for t in (kk, vv))
+    x = scale * np.einsum("hd,rhd->hr", qq, kk)
+    w = np.exp(x - x.max(1, keepdims=True))
+    w /= w.sum(1, keepdims=True)
+    out = np.einsum("hr,rhd->hd", w, vv)
+    size = np.log2(np.e) * abs(scale) * np.sqrt(np.einsum("hd,rhd->hr", qq ** 2, kk ** 2).max(1))
+    walk = np.einsum("hr,rhd->hd", w ** 2, (abs(vv) + abs(out)) ** 2)
+    may = ((7 * size + 8) * u)[:, None] ** 2 * walk + (4 * u * out) ** 2
+    return ((got.reshape(heads, -1) - out) ** 2).sum(), may.sum()
+
+
 def select(logits, score, done, codebook, eos, allow):
     """logits [requests, beams, vocab] -> score, token, parent, done [requests, beams]."""
     requests, beams, vocab = logits.shape

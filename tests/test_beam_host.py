@@ -208,6 +208,53 @@ def test_seen_rows():
     assert [ref.place(r, 2, 6) for r in range(11)] == [0, 1, 2, 3, 4, 5, 2, 3, 4, 5, 2]
 
 
+def planes(a, n, half=False):
+    """The first n 16-bit planes of a: bf16, or f16."""
+    left, got = np.asarray(a, np.float64), np.zeros_like(a, dtype=np.float64)
+    for _ in range(n):
+        if half:
+            part = left.astype(np.float16).astype(np.float64)
+        else:
+            bits = left.astype(np.float32).view(np.uint32).astype(np.uint64)
+            part = ((bits + 0x7fff + (bits >> 16 & 1)) & 0xffff0000).astype(np.uint32).view(np.float32).astype(np.float64)
+        got, left = got + part, left - part
+    return got
+
+
+@pytest.mark.parametrize("rows, hw", [(2, 128), (33, 72), (500, 72), (1399, 104), (2017, 128), (4096, 64)])
+def test_the_drift_that_is_allowed_tells_planes_apart(rows, hw):
+    """Results with one operand cut to fewer planes than the kernels keep are refused, whichever it is;
+    32-bit arithmetic is not."""
+    r = np.random.default_rng(rows)
+    lanes, scale = 12, 1.0 / np.sqrt(hw)
+    k, v = r.normal(size=(2, rows, hw)).astype(np.float32)
+    q = r.normal(size=(lanes, hw)).astype(np.float32)
+
+    def ratio(cut, n, half=False):
+        keep = {name: (lambda a, name=name: planes(a, n, half) if name == cut else np.asarray(a, np.float64)) for name in "qkwv"}
+        off = may = 0.0
+        for b in range(lanes):
+            x = scale * keep["k"](k) @ keep["q"](q[b])
+            w = np.exp(x - x.max())
+            out = keep["w"](w) @ keep["v"](v) / w.sum()
+            a, c = ref.drift(q[b], k, v, 1, scale, out)
+            off, may = off + a, may + c
+        return np.sqrt(off / may)
+
+    for cut in "qkwv":
+        assert ratio(cut, 1) > 100 and ratio(cut, 3) < 0.1, cut
+        assert ratio(cut, 1, half=True) > 10 and ratio(cut, 2, half=True) < 0.5, cut
+        if rows > 2:
+            assert ratio(cut, 2) > 1, cut
+    off = may = 0.0
+    for b in range(lanes):
+        x = (np.float32(scale) * q[b]) @ k.T
+        w = np.exp(x - x.max())
+        a, c = ref.drift(q[b], k, v, 1, scale, (w @ v / w.sum()).astype(np.float64))
+        off, may = off + a, may + c
+    assert off < may
+
+
 def test_selection_rules():
     x = np.log(np.array([[[4.0, 2.0, 1.0, 1.0], [1.0, 1.0, 5.0, 1.0]]], np.float32))
     score, token, parent, done = ref.select(x, np.zeros((1, 2), np.float32), np.zeros((1, 2), int), 3, 3, np.array([1]))

@@ -192,6 +192,36 @@ def test_prefix_tiles(tiled, kind, lanes, prefix, heads, hw):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("hw", [72, 104, 120, 128])
+@pytest.mark.parametrize("prefix", [1, 7, 31, 33, 64, 65])
+def test_prefix_tiles_of_wide_heads(tiled, kind, hw, prefix):
+    """Heads of two slabs behind few rows, where nothing averages out."""
+    attend(tiled, kind, 2, hw, [b % 4 for b in range(37)], 5, prefix_lengths=[prefix], seed=hw + prefix, prefix_spare=1, tiles=True)
+
+
+@pytest.mark.parametrize("walked", [False, True])
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("lanes, prefix, heads, hw", [(40, 4096, 3, 64), (40, 2017, 1, 128), (130, 500, 1, 72), (64, 1399, 5, 104),
+                                                      (24, 33, 3, 120), (24, 3000, 4, 32)])
+def test_the_drift_behind_a_prefix(kind, lanes, prefix, heads, hw, walked):
+    """All outputs together are as precise as operands of 24 (or 22) bits make them, which the bound of
+    a single output cannot tell behind many rows (test_beam_host: what it takes of fewer planes)."""
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("MYNAH_B200_LANE_TILES", "0" if walked else "1")
+        b = Backend("f32")
+    b.set_stream(torch.cuda.current_stream().cuda_stream)
+    x = attend(b, kind, heads, hw, [i % 4 for i in range(lanes)], 5, prefix_lengths=[prefix], seed=lanes + hw, tiles=not walked)
+    b.close()
+    out, off, may = x.d_out.cpu().numpy().astype(np.float64), 0.0, 0.0
+    for i in range(0, lanes, 3):
+        n, width = x.lengths[i], x.width
+        kk, vv = (np.concatenate([x.prefix[m][0, :prefix, :width], x.store[m][x.slots[i], :n + 1, :width]]) for m in "kv")
+        a, c = ref.drift(x.qkv[i, :width], kk, vv, heads, x.scale, out[i, :width])
+        off, may = off + a, may + c
+    assert off <= may, np.sqrt(off / may)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
 def test_tiles_of_several_prefixes(tiled, kind):
     """Two of them with more than one tile, one empty, one of a single row, lanes without any."""
     r = np.random.default_rng(8)
