@@ -533,9 +533,11 @@ typedef struct {
  * and the next mynah_cuda_sync reports it.  A slot may appear once per call.  Rows of the
  * cache that a lane does not see may hold anything.
  *
- * A prefix that enough lanes share is multiplied on the tensor cores, once for 128 lanes; the
- * environment, read when the backend is opened, overrides the choice: MYNAH_B200_LANE_TILES=0
- * (and MYNAH_B200_NO_TC=1) never, =1 for any 8 lanes.  Results agree to 32-bit rounding.
+ * A prefix that enough lanes share is multiplied on the tensor cores, once for 128 lanes, as far
+ * as lanes, heads, type and prefix_capacity tell (the lengths are on the device).  Sums stay
+ * 32-bit; of an f16 cache the query and the weights are kept in 22 bits, of an f32 one all operands
+ * in 24.  The environment, read when the backend is opened, overrides the choice:
+ * MYNAH_B200_LANE_TILES=0 (and MYNAH_B200_NO_TC=1) never, =1 for any 8 lanes.
  * Waits on the device are bounded: one that runs out makes the call's outputs stale and the next
  * mynah_cuda_sync report it.  MYNAH_B200_LANE_POLLS, read likewise, shortens them (tests).
  *

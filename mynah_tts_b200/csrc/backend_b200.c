@@ -345,7 +345,7 @@ int mynah_b200_open(void **state, int device, int quant, int strict, char *error
         mb_cuda(mb_cross_block_init(), "kernel attributes (cross-attention block)", error, cap) != 0 ||
         mb_cuda(mb_codec_tc_init(), "kernel attributes (codec tensor-core convolution)", error, cap) != 0 ||
         mb_cuda(mb_beam_init(st->beam_clusters), "kernel attributes (beam selection)", error, cap) != 0 ||
-        mb_cuda(mb_lane_attention_init(), "kernel attributes (lane attention)", error, cap) != 0 ||
+        mb_cuda(mb_lane_attention_init(&st->lane_device), "kernel attributes (lane attention)", error, cap) != 0 ||
         mb_cuda((int)cudaMalloc((void **)&st->d_token, sizeof(unsigned)), "cudaMalloc", error, cap) != 0 ||
         mb_cuda((int)cudaMalloc((void **)&st->d_status, 2u * sizeof(int)), "cudaMalloc", error, cap) != 0 ||
         mb_cuda((int)cudaMemset(st->d_status, 0, 2u * sizeof(int)), "cudaMemset", error, cap) != 0) {

@@ -148,6 +148,7 @@ int mynah_b200_lane_attention(void *state, const mynah_b200_lane_attention_args 
     m.sm_count = st->sm_count;
     m.tiles = st->lane_tiles;
     m.polls = st->lane_polls;
+    m.device = &st->lane_device;
     m.launched = &launched;
     device_scope scope;
     if (enter_device(st, &scope, error, cap) != 0) return -1;

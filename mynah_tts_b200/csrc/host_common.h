@@ -51,6 +51,7 @@ typedef struct mb_state {
     int libm_exact;                  /* 1 when both tables were built */
     int lane_tiles;                  /* prefixes of the lane attention on the tensor cores: 0 never, 1 always, -1 by size */
     unsigned lane_polls;             /* of a barrier of the lane attention, before a wait gives up */
+    mb_lane_device lane_device;
     int beam_clusters[9];            /* clusters of 1 .. 8 CTAs of the beam selection that fit the device */
     unsigned long long launches;
 } mb_state;

@@ -724,25 +724,35 @@ Shape lane_shape(size_t heads, size_t head_width, size_t size, int sm_count) {
 }
 
 // Whether the prefixes go through the tensor cores, from what the host knows: every lane's prefix
-// full, the lanes spread over the prefixes.  Walked like own rows they come from L2, at 14 (f32) and
-// 10 (f16) bytes a picosecond and some; a tile costs a launch, its queries and partials, 5 us, and 5
-// or 4 us for every block that its CTA takes one after the other.  With 12 heads of 64 and own rows
-// of 100 .. 300, tiles / walking: f32 24 lanes behind 4,000 rows 45.9 / 53.3 us, 16 lanes 43.8 / 40.2;
-// 48 behind 1,000 31.7 / 34.3, 32 lanes 28.7 / 26.2; 48 behind 217 25.5 / 19.4; f16 16 behind 4,000
-// 25.3 / 33.7, 12 lanes 21.9 / 25.2 (the estimate still walks), 8 lanes 21.5 / 19.7; 32 behind 1,000
-// 18.5 / 22.1, 16 lanes 19.0 / 17.5; 128 behind 217 32.5 / 29.7.
+// full (prefix_capacity: one far above the lengths in use picks tiles too early), the lanes spread over
+// the prefixes.  Walked like own rows they come from L2 and are bound by the arithmetic on groups of 16
+// columns per thread; as tiles they cost a start, so much for every block that a CTA takes one after
+// the other, and so much for every lane (its query, its partials, its own rows, which get fewer CTAs or
+// wait).  The figures are chosen to lose least on 957 pairs of times: 8 layouts of 256 to 1,536 columns,
+// 8 .. 256 lanes with 100 .. 300 own rows, prefixes of 100 .. 4,000; the rule takes a side more than 4% above
+// the other in 52 of them.  Tiles / walking, in us:
+//   12 x 64  f16: 32 lanes behind 1,000 rows 19.3 / 23.4, 16 lanes 18.8 / 16.8; 128 behind 217 31.0 / 29.4
+//            f32: 64 lanes behind 1,000 rows 35.0 / 43.5, 32 lanes 28.3 / 27.1; 128 behind 217 43.8 / 37.3
+//   8 x 96   f16: 32 lanes behind 1,000 rows 25.8 / 36.3, 8 lanes 17.0 / 14.2; f32: 64 lanes 43.7 / 59.9, 16 lanes 26.5 / 23.9
+//   6 x 128  f16: 32 lanes behind 1,000 rows 23.4 / 26.0, 16 lanes 17.6 / 15.2; f32: 64 lanes 41.7 / 44.4, 32 lanes 32.4 / 30.4
 constexpr size_t TILE_LANES = 8;   // fewer lanes never use them (and have no workspace for them)
 
+struct TileCost { double start_us, turn_us, lane_us, bytes_per_us; };      // lane_us: of 768 columns
+constexpr TileCost TILE_COST[2][2] = {{{0.0, 3.5, 0.03, 25e6}, {4.0, 2.5, 0.04, 22e6}},    // f32: heads up to 64, wider
+                                      {{0.0, 2.5, 0.02, 18e6}, {1.5, 2.0, 0.02, 22e6}}};   // f16
+
 bool use_tiles(size_t lanes, size_t heads, size_t head_width, size_t size, size_t prefixes, size_t prefix_capacity, size_t window,
-               size_t sinks, int sm_count) {
+               size_t sinks, int lpr, size_t at_once) {
     if (prefixes == 0 || lanes < TILE_LANES) return false;
     const bool f16 = size == 2u;
+    const TileCost cost = TILE_COST[f16][head_width > 64];
     const size_t seen = window > 0 && window + sinks < prefix_capacity ? window + sinks : prefix_capacity;
     const size_t full = (lanes + TILE - 1) / TILE, tiles = prefixes > full ? (prefixes < lanes ? prefixes : lanes) : full;
-    const size_t keys = f16 ? TileShape<__half, 1>::KEYS : TileShape<float, 1>::KEYS, at_once = (size_t)(TILE_CTAS_PER_SM * sm_count);
+    const size_t keys = f16 ? TileShape<__half, 1>::KEYS : TileShape<float, 1>::KEYS;
     const size_t blocks = tiles * heads * ((prefix_capacity + keys - 1) / keys), turns = (blocks + at_once - 1) / at_once;
-    const double walk_us = 2.0 * (double)(lanes * seen) * (double)(heads * head_width * size) / (f16 ? 10e6 : 14e6);
-    return walk_us > 5.0 + (f16 ? 4.0 : 5.0) * (double)turns;
+    const double columns = (double)(lanes * heads * (size_t)lpr * 16u);
+    const double walk_us = 2.0 * (double)seen * columns * (double)size / cost.bytes_per_us;
+    return walk_us > cost.start_us + cost.turn_us * (double)turns + cost.lane_us * columns / 768.0;
 }
 
 // Places of the workspace, in floats.
@@ -783,15 +793,41 @@ int with_rows_kernel(int lpr, bool full, F f) {
 size_t rows_smem(size_t lanes, const Shape &s) {
     return ((lanes + 1u) * 4u + 15u) / 16u * 16u + (size_t)ROWS_DEPTH * 2u * (size_t)s.step * (size_t)s.row_pitch;
 }
+// How many CTAs of the prefix tiles an SM holds, TILE_CTAS_PER_SM at most, and whether one of the
+// rows fits beside them.
+struct TileFit { int ctas; bool beside; };
+
+size_t tile_smem(size_t size, size_t head_width, size_t lanes, size_t prefixes) {
+    const size_t operands = size == 2u ? (head_width <= 64 ? TileShape<__half, 1>::SMEM : TileShape<__half, 2>::SMEM)
+                                       : (head_width <= 64 ? TileShape<float, 1>::SMEM : TileShape<float, 2>::SMEM);
+    return operands + 16u * prefixes + 6u * lanes + 16u;
+}
+
+TileFit tile_fit(const mb_lane_device &device, const Shape &s, size_t size, size_t head_width, size_t lanes, size_t prefixes) {
+    const auto &tile = device.tiles[size == 2u][head_width > 64];
+    const size_t reserved = 1024u;                         // shared memory that a CTA takes besides its own
+    const size_t smem = tile.smem + tile_smem(size, head_width, lanes, prefixes) + reserved, registers = tile.registers * TILE;
+    TileFit fit = {TILE_CTAS_PER_SM, false};
+    while (fit.ctas > 1 && (fit.ctas * smem > device.smem || fit.ctas * registers > device.registers)) --fit.ctas;
+    const size_t threads = (size_t)(s.heads_per_cta * s.phases + 1) * 32u;
+    fit.beside = fit.ctas * smem + device.rows.smem + rows_smem(lanes, s) + reserved <= device.smem &&
+                 fit.ctas * registers + device.rows.registers * threads <= device.registers;
+    return fit;
+}
+// Whether the rows are cut for one CTA per SM instead of two.  f32 tiles last longer than what one gains
+// beside them meanwhile, also where it fits (8 x 96, 64 lanes behind 1,000 rows: 44.1 us with runs for two, 56.1 for
+// one; 12 x 64, 48 lanes 31.7 / 33.9).  Beside f16 tiles one fits where heads are up to 64 (12 x 64, 32
+// lanes behind 1,000: 21.6 / 18.5; 16 behind 4,000 27.2 / 25.3; where the own rows go on for as long as
+// the tiles, 256 lanes of up to 500 behind 4,096, 73.3 / 74.6).  Wider ones take nearly all registers, so
+// that the rows follow them: runs for two where they are of 8 steps or more (8 x 96, 64 lanes of up to 300
+// behind 1,000: 33.9 / 35.2, 256 of up to 2,000 behind 4,000 212 / 362; 6 x 128, 64 lanes of up to 2,000 63 / 78, of
+// up to 300 30.8 / 28.5), as far as the capacity tells.
+bool one_rows_cta(const TileFit &fit, const Shape &s, size_t size, size_t lanes, size_t capacity) {
+    return size == 2u && (fit.beside || lanes * capacity < 8u * (size_t)s.step * (size_t)s.workers);
+}
 template <typename T>
-int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
-    // Beside two f16 CTAs of k_lane_prefix an SM has room for one CTA of this: runs for one CTA per SM
-    // (32 lanes behind 1,000 rows: 18.5 us against 21.6; 16 behind 4,000: 25.3 / 27.2; where the own rows
-    // go on for as long as the tiles, 256 lanes of up to 500 behind 4,096, it is 74.6 / 73.3).  Beside
-    // two f32 ones it has none, and takes two when they have ended (48 lanes behind 1,000: 31.7 us
-    // against 33.9 with runs for one).
-    const bool beside = p.tile_workers > 0 && sizeof(T) == 2;
-    const int workers = beside && s.workers > 1 ? s.workers / CTAS_PER_SM : s.workers;
+int launch_rows(const LaneP &p, const Shape &s, bool one_per_sm, cudaStream_t stream) {
+    const int workers = one_per_sm && s.workers > 1 ? s.workers / CTAS_PER_SM : s.workers;
     const dim3 grid((unsigned)workers, (unsigned)s.groups), block((unsigned)((s.heads_per_cta * s.phases + 1) * 32));
     return with_rows_kernel<T>(s.lpr, p.head_width == s.lpr * 16, [&](auto kernel) {
         return mb_launch(kernel, grid, block, rows_smem((size_t)p.lanes, s), stream, p);
@@ -799,23 +835,19 @@ int launch_rows(const LaneP &p, const Shape &s, cudaStream_t stream) {
 }
 
 template <typename T, int SLABS>
-size_t tile_smem(size_t lanes, size_t prefixes) {
-    return TileShape<T, SLABS>::SMEM + 16u * prefixes + 6u * lanes + 16u;
-}
-template <typename T, int SLABS>
 int launch_tiles(const LaneP &p, cudaStream_t stream) {
-    return mb_launch(k_lane_prefix<T, SLABS>, dim3((unsigned)p.tile_workers), dim3(TILE), tile_smem<T, SLABS>((size_t)p.lanes, p.prefixes),
-                     stream, p);
+    return mb_launch(k_lane_prefix<T, SLABS>, dim3((unsigned)p.tile_workers), dim3(TILE),
+                     tile_smem(sizeof(T), (size_t)p.head_width, (size_t)p.lanes, p.prefixes), stream, p);
 }
 
 template <typename T>
-int launch_all(const LaneP &p, const Shape &s, int sm_count, cudaStream_t stream, unsigned *launched) {
+int launch_all(const LaneP &p, const Shape &s, bool one_per_sm, int sm_count, cudaStream_t stream, unsigned *launched) {
     int rc = 0;
     if (p.tile_workers > 0) {
         rc = p.head_width <= 64 ? launch_tiles<T, 1>(p, stream) : launch_tiles<T, 2>(p, stream);
         if (rc != 0) return rc;
     }
-    rc = launch_rows<T>(p, s, stream);
+    rc = launch_rows<T>(p, s, one_per_sm, stream);
     if (rc != 0) return rc;
     int columns = 1;
     while (columns * 4 < p.head_width) columns *= 2;
@@ -837,7 +869,7 @@ extern "C" size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t he
     return lane_places(lanes, heads, head_width, prefixes, sm_count).floats;
 }
 
-extern "C" int mb_lane_attention_init(void) {
+extern "C" int mb_lane_attention_init(mb_lane_device *device) {
     const auto allow = [](auto kernel, size_t smem) {
         return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     };
@@ -849,10 +881,28 @@ extern "C" int mb_lane_attention_init(void) {
             if (rc == 0) rc = with_rows_kernel<float>(lpr, full, [&](auto k) { return allow(k, ROWS_SMEM_MOST); });
             if (rc == 0) rc = with_rows_kernel<__half>(lpr, full, [&](auto k) { return allow(k, ROWS_SMEM_MOST); });
         }
-    if (rc == 0) rc = allow(k_lane_prefix<float, 1>, tile_smem<float, 1>(MB_LANES_MAX, MB_LANES_MAX));
-    if (rc == 0) rc = allow(k_lane_prefix<float, 2>, tile_smem<float, 2>(MB_LANES_MAX, MB_LANES_MAX));
-    if (rc == 0) rc = allow(k_lane_prefix<__half, 1>, tile_smem<__half, 1>(MB_LANES_MAX, MB_LANES_MAX));
-    if (rc == 0) rc = allow(k_lane_prefix<__half, 2>, tile_smem<__half, 2>(MB_LANES_MAX, MB_LANES_MAX));
+    int current = 0, smem = 0, registers = 0;
+    if (rc == 0) rc = (int)cudaGetDevice(&current);
+    if (rc == 0) rc = (int)cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerMultiprocessor, current);
+    if (rc == 0) rc = (int)cudaDeviceGetAttribute(&registers, cudaDevAttrMaxRegistersPerMultiprocessor, current);
+    device->smem = (size_t)smem;
+    device->registers = (size_t)registers;
+    const auto takes = [](auto kernel, auto &what) {
+        cudaFuncAttributes at;
+        const int error = (int)cudaFuncGetAttributes(&at, kernel);
+        what.smem = at.sharedSizeBytes;
+        what.registers = ((size_t)at.numRegs + 7u) / 8u * 8u;
+        return error;
+    };
+    if (rc == 0) rc = takes(k_lane_rows<__half, 4, true>, device->rows);      // all variants: __maxnreg__, the same arrays
+    const auto tiles = [&](auto kernel, size_t size, size_t head_width) {
+        const int error = takes(kernel, device->tiles[size == 2u][head_width > 64u]);
+        return error != 0 ? error : allow(kernel, tile_smem(size, head_width, MB_LANES_MAX, MB_LANES_MAX));
+    };
+    if (rc == 0) rc = tiles(k_lane_prefix<float, 1>, 4u, 64u);
+    if (rc == 0) rc = tiles(k_lane_prefix<float, 2>, 4u, 128u);
+    if (rc == 0) rc = tiles(k_lane_prefix<__half, 1>, 2u, 64u);
+    if (rc == 0) rc = tiles(k_lane_prefix<__half, 2>, 2u, 128u);
     return rc;
 }
 
@@ -899,18 +949,20 @@ extern "C" int mb_lane_attention(const mb_lane_attn_args *a, mb_stream stream) {
     p.step = s.step;
     p.row_bytes = s.row_bytes;
     p.row_pitch = s.row_pitch;
+    const size_t size = a->cache.type == MB_F16 ? 2u : 4u;
+    const TileFit fit = tile_fit(*a->device, s, size, a->head_width, a->lanes, a->prefixes);
     bool tiles = a->tiles > 0 && a->prefixes > 0 && a->lanes >= TILE_LANES;
     if (a->tiles < 0)
-        tiles = use_tiles(a->lanes, a->heads, a->head_width, a->cache.type == MB_F16 ? 2u : 4u, a->prefixes, a->prefix_capacity,
-                          a->window, a->sinks, a->sm_count);
-    if (tiles)
-        p.tile_workers = TILE_CTAS_PER_SM * a->sm_count;
+        tiles = use_tiles(a->lanes, a->heads, a->head_width, size, a->prefixes, a->prefix_capacity, a->window, a->sinks, s.lpr,
+                          (size_t)(fit.ctas * a->sm_count));
+    if (tiles) p.tile_workers = fit.ctas * a->sm_count;
     p.tile_lane = reinterpret_cast<unsigned *>(a->workspace + w.tile_lane);
     p.tile_prefix = reinterpret_cast<uint4 *>(a->workspace + w.tile_prefix);
     p.tile_run = reinterpret_cast<unsigned *>(a->workspace + w.tile_run);
     p.tile_stat = reinterpret_cast<float2 *>(a->workspace + w.tile_stat);
     p.tile_acc = a->workspace + w.tile_acc;
     const cudaStream_t st = (cudaStream_t)stream;
-    return a->cache.type == MB_F16 ? launch_all<__half>(p, s, a->sm_count, st, a->launched)
-                                   : launch_all<float>(p, s, a->sm_count, st, a->launched);
+    const bool one_per_sm = tiles && one_rows_cta(fit, s, size, a->lanes, a->cache.capacity);
+    return a->cache.type == MB_F16 ? launch_all<__half>(p, s, one_per_sm, a->sm_count, st, a->launched)
+                                   : launch_all<float>(p, s, one_per_sm, a->sm_count, st, a->launched);
 }

@@ -402,6 +402,7 @@ typedef struct {
 } mb_beam_reorder_args;
 int mb_beam_reorder(const mb_beam_reorder_args *args, mb_stream stream);
 
+typedef struct mb_lane_device mb_lane_device;
 enum { MB_LANES_MAX = 1024, MB_LANE_HEADS_MAX = 64, MB_LANE_HEAD_WIDTH_MAX = 128 };
 typedef struct {
     size_t lanes, heads, head_width;
@@ -424,11 +425,17 @@ typedef struct {
     int sm_count;
     int tiles;                  /* prefixes on the tensor cores: 0 never, 1 wherever possible, -1 where faster */
     unsigned polls;             /* of a device barrier, before a wait gives up and sets status */
+    const mb_lane_device *device;       /* mb_lane_attention_init's */
     unsigned *launched;         /* incremented by the number of kernels the call enqueued */
 } mb_lane_attn_args;
 enum { MB_LANE_POLLS = 1 << 24 };   /* seconds */
+/* What an SM of the current device holds, and what the prefix tiles and the rows take of it. */
+struct mb_lane_device {
+    size_t smem, registers;
+    struct { size_t smem, registers; } tiles[2][2], rows;   /* static bytes, registers per thread; [f32, f16][64, 128 columns] */
+};
 size_t mb_lane_attention_floats(size_t lanes, size_t heads, size_t head_width, size_t prefixes, int sm_count);
-int mb_lane_attention_init(void);
+int mb_lane_attention_init(mb_lane_device *device);
 int mb_lane_attention(const mb_lane_attn_args *args, mb_stream stream);
 
 #ifdef __cplusplus

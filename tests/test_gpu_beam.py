@@ -318,6 +318,25 @@ def test_the_choice_of_tiles(be, tiled):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("heads, hw", [(8, 96), (6, 128), (12, 128), (4, 80), (8, 64)])
+def test_tiles_and_rows_that_share_an_sm_or_follow(tiled, kind, heads, hw):
+    """Layouts of which one or two tile CTAs fit on an SM, with or without one of the rows; own rows
+    that go on for longer than the tiles, and more blocks than CTAs."""
+    r = np.random.default_rng(hw)
+    attend(tiled, kind, heads, hw, [int(n) for n in r.integers(0, 700, 40)], 701, prefix_lengths=[900], seed=hw, tiles=True)
+    attend(tiled, kind, heads, hw, [int(n) for n in r.integers(0, 4, 200)], 4, prefix_lengths=[1500, 40],
+           voices=[int(v) for v in r.integers(0, 3, 200)], seed=heads, tiles=True)
+
+
+def test_the_choice_of_tiles_for_wide_heads(be):
+    """A tile CTA of f32 heads above 64 has an SM to itself: half the blocks at a time."""
+    r = np.random.default_rng(2)
+    for kind, hw, lanes, prefix, tiles in (("f16", 128, 64, 2000, True), ("f16", 128, 9, 200, False), ("f32", 128, 64, 2000, True),
+                                           ("f32", 128, 16, 500, False), ("f32", 96, 40, 2000, True), ("f16", 80, 12, 300, False)):
+        attend(be, kind, 6, hw, [int(n) for n in r.integers(0, 4, lanes)], 4, prefix_lengths=[prefix], seed=hw, tiles=tiles)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("lanes, prefixes", [(300, 70), (1024, 1024)])
 def test_tiles_of_many_prefixes(tiled, kind, lanes, prefixes):
     """More prefixes than a warp has lanes; most tiles hold a few lanes, some prefixes none."""
