@@ -162,9 +162,9 @@ __device__ __forceinline__ float sel_exp(float x, float top) {
 // exp(x - top), 1 for nothing on both sides
 __device__ __forceinline__ float sel_scale(float x, float top) { return x == top ? 1.0f : sel_exp(x, top); }
 
-// log(s) for a positive normal s, to 1e-12: with s = 2^e f and c near 1 / f in steps of 1/256
+// log(s) for a positive normal s, to 1e-11: with s = 2^e f and c near 1 / f in steps of 1/256
 // (64 intervals of f, Tang's table method), log s = e log 2 - log c + log(1 + r), r = f c - 1, |r| <
-// 0.013.  r is formed in 64 bits; of log(1 + r) = r - r^2/2 + ... only r needs them.  CUDA's
+// 0.013.  r is formed in 64 bits; of log(1 + r) = r - r^2/2 + ... the rest is, in 32 bits, off by 9e-12.  CUDA's
 // 64-bit log took 1.7 us here, which the whole cluster waits for; this takes a tenth.
 __constant__ double sel_log_c[64] = {      // -log(c), c = round(256 / (1 + (i + 0.5) / 64)) / 256
     0.007843177461025893, 0.023716526617316044, 0.039845908547199674, 0.05211600113901402,
@@ -704,7 +704,9 @@ __global__ void __launch_bounds__(FIT ? SEL_FIT_THREADS : SEL_THREADS, FIT ? 4 :
 // so neither a cycle of parents nor a beam that several others follow needs a second buffer,
 // and a parent's row that several beams take comes from memory once.  Beams that keep their
 // own rows move nothing.  12 layers of 768 columns, 16 requests of 4 beams, f16, 332 MB: 60 us, 5.5
-// TB/s; 4 requests of 8 beams, f32, 1.6 GB: 279 us, 5.75 TB/s, 85 and 89% of what a plain copy reaches.
+// TB/s; 4 requests of 8 beams, f32, 1.6 GB: 279 us, 5.75 TB/s, 85 and 89% of what a plain copy reaches; 4 of 16
+// beams, f32, 1.7 GB 289 us, 5.8 TB/s.  A warp takes a row, so rows below 512 bytes leave lanes of it idle: 64
+// requests of 4 beams with rows of 256 bytes 3.2 TB/s, of 64 bytes 0.9.
 
 struct ReorderP {
     char *k, *v;
@@ -877,7 +879,8 @@ extern "C" int mb_beam_reorder(const mb_beam_reorder_args *a, mb_stream stream) 
     p.length = a->length;
     p.length_out = a->length_out;
     p.live = a->live;
-    // eight CTAs per SM where there is that much work; a CTA walks its plane's rows
+    // a grid of eight CTAs per SM where there is that much work, of which three, two or one are resident at a
+    // time (70, 102 or 176 registers a thread for 4, 8 or 16 beams); a CTA walks its plane's rows
     const size_t want = 8u * (size_t)a->sm_count, have = (size_t)p.planes * a->requests;
     size_t x = (want + have - 1u) / have, most = (a->cache.capacity + 7u) / 8u;
     if (x > most) x = most;

@@ -670,7 +670,8 @@ __global__ void __launch_bounds__(WARPS == 1 ? MERGE_HEADS * 32 : WARPS * 32) k_
         if (s_again == 0) return;
     }
     // Infinities or NaN among the rows: a value kept as planes turns inf into inf - inf, so this
-    // head is formed once more from the values themselves, row by row.
+    // head is formed once more from the values themselves, row by row (slowly: 256 lanes behind 4,096 rows,
+    // one infinite value in a head of which 1.6 ms).
     const size_t prefix = (size_t)w.prefix * p.prefix_stride + head * p.head_width + d;
     const size_t slot = w.slot * p.slot_stride + head * p.head_width + d;
     r = slice == 0 && x != -INFINITY ? own : none;
@@ -873,8 +874,9 @@ extern "C" int mb_lane_attention_init(mb_lane_device *device) {
     const auto allow = [](auto kernel, size_t smem) {
         return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     };
-    // a step of one phase may be above ROWS_STAGE: 12 heads of 128 f32 elements are 4 rows of 6 KB
-    constexpr size_t ROWS_SMEM_MOST = (MB_LANES_MAX + 4u) * 4u + ROWS_DEPTH * (ROWS_STAGE + 16u * 1024u);
+    // steps of one phase are within ROWS_STAGE too: 12 heads of 64 f32 columns are 8 rows of 3,136 bytes, of K and
+    // of V; 12 of 32 f16 columns, 32 of 800, are the most
+    constexpr size_t ROWS_SMEM_MOST = (MB_LANES_MAX + 4u) * 4u + ROWS_DEPTH * ROWS_STAGE;
     int rc = 0;
     for (int lpr = 1; lpr <= 8; lpr *= 2)
         for (int full = 0; full < 2; ++full) {

@@ -555,6 +555,12 @@ def test_many_lanes(be):
            voices=[int(v) for v in r.integers(0, 2, 1024)], seed=11)
 
 
+@pytest.mark.parametrize("kind, heads, hw", [("f32", 6, 64), ("f16", 12, 32), ("f32", 12, 128)])
+def test_the_largest_rings(be, kind, heads, hw):
+    """Layouts whose steps fill the rows' ring, beside the schedule of the most lanes."""
+    attend(be, kind, heads, hw, [b % 3 for b in range(1024)], 3, prefix_lengths=[2], seed=16)
+
+
 def test_offsets_beyond_32_bits(be):
     """Slots more than 2^32 elements into the cache."""
     heads, hw, capacity = 2, 128, 2 ** 17
