@@ -537,7 +537,7 @@ class Decoder:
         lives in slots[lane] and continues beam parents[lane] of its request."""
         slots = np.ascontiguousarray(slots, np.uint32)
         parents = np.ascontiguousarray(parents, np.uint32)
-        if slots.ndim != 1 or slots.shape != parents.shape or slots.size % beams != 0:
+        if beams < 1 or slots.ndim != 1 or slots.shape != parents.shape or slots.size % beams != 0:
             raise ValueError("slots and parents hold requests * beams entries each")
         call(capi.lib().mynah_b200_decoder_reorder, self.handle, slots.ctypes.data_as(capi.c_uint_p),
              parents.ctypes.data_as(capi.c_uint_p), slots.size // beams, beams)

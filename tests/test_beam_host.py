@@ -11,7 +11,7 @@ import pytest
 
 import beam_reference as ref
 from mynah_tts_b200 import capi
-from mynah_tts_b200.backend import Backend
+from mynah_tts_b200.backend import Backend, Decoder
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 STATE = C.create_string_buffer(4096)
@@ -144,6 +144,13 @@ def test_decoder_reorder_refuses_rows_that_are_not_16_byte_pieces():
     two = (C.c_uint * 2)(0, 1)
     assert capi.lib().mynah_b200_decoder_reorder(decoder, two, two, 1, 2, err, capi.ERR_CAP) == -1
     assert b"multiples of 4" in err.value
+
+
+@pytest.mark.parametrize("slots, parents, beams", [([0, 1], [0, 0], 0), ([0, 1], [0, 0], -1), ([0, 1, 2], [0, 0, 0], 2),
+                                                   ([0, 1], [0], 2), ([[0, 1]], [[0, 0]], 2)])
+def test_decoder_reorder_refuses_other_shapes(slots, parents, beams):
+    with pytest.raises(ValueError, match="requests \\* beams"):
+        Decoder.reorder(Decoder.__new__(Decoder), slots, parents, beams)
 
 
 def test_bound_calls_report_a_refusal():
