@@ -236,7 +236,8 @@ class Backend:
 
     def bind_beam_reorder(self, cache: capi.LaneCache, *, requests: int, beams: int, parent, length, length_out=None,
                           slot=None, live=None):
-        """The picked beams' own rows, in place."""
+        """The picked beams' own rows, in place: the first length[parent] of them, which behind a step's
+        lane_attention are its length + 1; length_out receives the next step's lengths."""
         args = capi.BeamReorderArgs(cache, requests, beams, _a(slot), _a(parent), _a(length), _a(length_out), _a(live))
         return self._bound(self.lib.mynah_b200_beam_reorder, args)
 

@@ -148,6 +148,8 @@ struct Piece<__half> {
     }
 };
 
+// 2^x, off by at most 2^-22 of itself: one instruction per row, head and thread.  A weight carries as
+// much from its score, whose 32-bit sum is off by a few 2^-24 of a value of 1 to 10.
 __device__ __forceinline__ float pow2(float x) {
     float y;
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
