@@ -356,7 +356,9 @@ int mynah_b200_open(void **state, int device, int quant, int strict, char *error
     {
         const char *no_tc = getenv("MYNAH_B200_NO_TC"), *tiles = getenv("MYNAH_B200_LANE_TILES"), *polls = getenv("MYNAH_B200_LANE_POLLS");
         st->lane_tiles = no_tc != NULL && strcmp(no_tc, "0") != 0 ? 0 : tiles != NULL ? strcmp(tiles, "0") != 0 : -1;
-        st->lane_polls = polls != NULL && strtoul(polls, NULL, 10) < MB_LANE_POLLS ? (unsigned)strtoul(polls, NULL, 10) : MB_LANE_POLLS;
+        char *end = NULL;
+        const unsigned long n = polls != NULL ? strtoul(polls, &end, 10) : MB_LANE_POLLS;
+        st->lane_polls = n < MB_LANE_POLLS && end != polls && *end == '\0' ? (unsigned)n : MB_LANE_POLLS;
     }
     if (st->strict) {
         const char *env = getenv("MYNAH_B200_LIBM_TABLES");

@@ -731,7 +731,7 @@ Shape lane_shape(size_t heads, size_t head_width, size_t size, int sm_count) {
 // the prefixes.  Walked like own rows they come from L2 and are bound by the arithmetic on groups of 16
 // columns per thread; as tiles they cost a start, so much for every block that a CTA takes one after
 // the other, and so much for every lane (its query, its partials, its own rows, which get fewer CTAs or
-// wait).  The figures are chosen to lose least on 957 pairs of times: 8 layouts of 256 to 1,536 columns,
+// wait).  The figures are chosen to lose least on 958 pairs of times: 8 layouts of 256 to 1,536 columns,
 // 8 .. 256 lanes with 100 .. 300 own rows, prefixes of 100 .. 4,000; the rule takes a side more than 4% above
 // the other in 52 of them.  Tiles / walking, in us:
 //   12 x 64  f16: 32 lanes behind 1,000 rows 19.3 / 23.4, 16 lanes 18.8 / 16.8; 128 behind 217 31.0 / 29.4

@@ -549,6 +549,16 @@ def test_waits_that_run_out_are_reported(be, kind, heads, hw, lanes, tiles, poll
     y.check()
 
 
+@pytest.mark.parametrize("polls", ["", "many", "-1", "3 ", "99999999999999999999"])
+def test_a_wait_that_is_no_number_is_the_default(polls):
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("MYNAH_B200_LANE_POLLS", polls)
+        b = Backend("f32")
+    b.set_stream(torch.cuda.current_stream().cuda_stream)
+    attend(b, "f32", 2, 64, [300, 0, 40], 301, prefix_lengths=[30], seed=17)
+    b.close()
+
+
 def test_many_lanes(be):
     r = np.random.default_rng(11)
     attend(be, "f16", 1, 32, [int(n) for n in r.integers(0, 12, 1024)], 12, prefix_lengths=[9, 140],
@@ -761,6 +771,27 @@ def test_select_of_equal_beams_at_every_alignment(be, beams, vocab):
         rows = r.normal(0, 2, (requests, 1, vocab)).astype(np.float32)
         check_select(be, np.repeat(rows, beams, 1), np.repeat(-20 * r.random((requests, 1)), beams, 1), None, vocab, vocab, None,
                      stride=stride, offset=stride % 3)
+
+
+@pytest.mark.parametrize("beams, vocab", [(3, 61), (8, 2016), (2, 20011), (16, 9001)])
+def test_select_of_equal_beams_with_an_end_gaps_and_flags(be, beams, vocab):
+    """Equal beams whose end token counts in the sum, whose rows hold NaN and -inf, some of them done, with
+    scores and flags overwritten; and finished ones level with a beam that has one token left."""
+    r = np.random.default_rng(vocab)
+    row = r.normal(0, 2, vocab).astype(np.float32)
+    row[r.integers(0, vocab - 8, vocab // 9)] = np.nan
+    row[r.integers(0, vocab - 8, vocab // 9)] = -np.inf
+    row[vocab - 1] = np.nanmax(row) - 0.5
+    logits = np.repeat(np.stack([row, r.permutation(row)])[:, None], beams, 1)
+    logits[1, :, vocab - 1] = np.nan
+    done = np.zeros((2, beams), np.int64)
+    done[:, 1] = 1
+    score = np.full((2, beams), -2.5, np.float32)
+    for stride in (vocab, vocab + 1):
+        check_select(be, logits, score, done, vocab - 7, vocab - 1, np.array([1, 1]), stride=stride, offset=1, in_place=True)
+    only = np.full((2, beams, vocab), -np.inf, np.float32)
+    only[:, :, 5] = 3.25
+    check_select(be, only, score, done, vocab - 7, vocab - 1, np.array([1, 0]), stride=vocab + 3)
 
 
 @pytest.mark.parametrize("vocab", [2016, 20011])
